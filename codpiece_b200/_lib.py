@@ -10,7 +10,7 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libcpq.so"
 
-TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K = 0, 1, 8, 12, 14, 15
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K, TYPE_Q8_K, TYPE_BF16 = 0, 1, 8, 12, 14, 15, 30
 
 STATUS = {
     0: "CPQ_SUCCESS",
@@ -28,6 +28,8 @@ EXPORTED = [
     "cpq_init", "cpq_release", "cpq_mul_mat_workspace_size", "cpq_mul_mat", "cpq_mul_mat_ws",
     "cpq_mul_mat_multi", "cpq_mul_mat_fused", "cpq_mul_mat_noalloc", "cpq_quantize_act", "cpq_rms_norm",
     "cpq_swiglu", "cpq_add_inplace", "cpq_argmax", "cpq_gated_delta_net",
+    "cpq_rope_create", "cpq_rope_destroy", "cpq_rope_apply", "cpq_kv_slots", "cpq_kv_append", "cpq_kv_gather",
+    "cpq_paged_attn_workspace_size", "cpq_paged_attn",
     "cpq_decode_plan_create", "cpq_decode_plan_run", "cpq_decode_plan_destroy",
     "cpq_trunk_create", "cpq_trunk_run", "cpq_trunk_phases", "cpq_trunk_destroy",
     "cpq_gguf_open", "cpq_gguf_close", "cpq_gguf_n_tensors", "cpq_gguf_find_tensor", "cpq_gguf_tensor_at",
@@ -73,6 +75,31 @@ class CpqGgufTensor(C.Structure):
                 ("offset", C.c_uint64), ("bytes", C.c_uint64)]
 
 
+class CpqRopeParams(C.Structure):
+    _fields_ = [("n_dims", C.c_int32), ("mode", C.c_int32), ("base", C.c_double), ("freq_scale", C.c_double),
+                ("ext_factor", C.c_double), ("attn_factor", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("n_ctx_orig", C.c_int64), ("freq_factors", C.POINTER(C.c_double))]
+
+
+class CpqKvCache(C.Structure):
+    _fields_ = [("format", C.c_int32), ("head_dim", C.c_int32), ("n_head_kv", C.c_int32), ("block", C.c_int32),
+                ("n_pages", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p)]
+
+
+class CpqKvSlotArgs(C.Structure):
+    _fields_ = [("ctx_len", C.c_void_p), ("new_len", C.c_void_p), ("n_seqs", C.c_int64), ("table", C.c_void_p),
+                ("table_stride", C.c_int64), ("max_blocks", C.c_int32), ("block", C.c_int32),
+                ("free_pages", C.c_void_p), ("n_free", C.c_int64), ("taken", C.c_void_p), ("taken_out", C.c_void_p),
+                ("seq_start", C.c_void_p), ("kv_len", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p),
+                ("n_rows", C.c_int64)]
+
+
+class CpqAttnSeqs(C.Structure):
+    _fields_ = [("seq_start", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_int64),
+                ("n_seqs", C.c_int64), ("max_blocks", C.c_int32)]
+
+
 PRO_NONE, PRO_RMS, PRO_SWIGLU = 0, 1, 2
 
 
@@ -110,6 +137,15 @@ def lib() -> C.CDLL:
         "cpq_add_inplace": (st, [vp, vp, i64, vp]),
         "cpq_argmax": (st, [vp, i64, i64, vp, vp]),
         "cpq_gated_delta_net": (st, [P(CpqTensor)] * 7 + [C.c_int32, vp, i64, vp]),
+        "cpq_rope_create": (st, [P(CpqRopeParams), P(vp)]),
+        "cpq_rope_destroy": (None, [vp]),
+        "cpq_rope_apply": (st, [vp, P(P(CpqTensor)), P(P(CpqTensor)), C.c_int, vp, vp]),
+        "cpq_kv_slots": (st, [P(CpqKvSlotArgs), vp]),
+        "cpq_kv_append": (st, [P(CpqKvCache), P(CpqTensor), P(CpqTensor), vp, vp]),
+        "cpq_kv_gather": (st, [P(CpqKvCache), vp, P(CpqTensor), P(CpqTensor), vp]),
+        "cpq_paged_attn_workspace_size": (sz, [P(CpqKvCache), P(CpqTensor)]),
+        "cpq_paged_attn": (st, [P(CpqTensor), P(CpqKvCache), P(CpqAttnSeqs), C.c_float, i32, P(CpqTensor), vp, vp, sz,
+                                vp]),
         "cpq_decode_plan_create": (st, [P(CpqDecodePhase), C.c_int, C.c_int, P(vp)]),
         "cpq_decode_plan_run": (st, [vp, vp]),
         "cpq_decode_plan_destroy": (None, [vp]),

@@ -14,6 +14,9 @@
 //   decode.cuh       persistent decode step: a chain of Q4_K GEMV phases in one launch
 //   trunk.cuh        persistent decode trunk: every layer of a rank's step in one launch
 //   gdn.cuh          gated delta-net recurrence (the GDN layers' per-token state update)
+//   rope.cuh         rotary positions
+//   kv_cache.cuh     paged 8-bit key/value cache: slot maps, append, gather
+//   paged_attn.cuh   attention over the paged cache
 //   elementwise.cuh  rms norm, SwiGLU, residual add, argmax
 //   synth.cuh        seeded synthetic weights
 //   split.inl        tensor-parallel partition rules (host)
@@ -25,6 +28,9 @@
 //   trunk.inl        cpq_trunk_*: host side of the persistent decode trunk
 //   gguf.inl         cpq_gguf_*: GGUF reader and tensor-parallel shard loader (host)
 //   gdn.inl          cpq_gated_delta_net: host side of gdn.cuh
+//   rope.inl         cpq_rope_*: frequencies and host side of rope.cuh
+//   kv_cache.inl     cpq_kv_*: host side of kv_cache.cuh
+//   paged_attn.inl   cpq_paged_attn: host side of paged_attn.cuh
 #if defined(__CUDA_ARCH__) && __CUDA_ARCH__ < 1000
 #error "libcpq targets sm_100a (B200) only"
 #endif
@@ -47,6 +53,9 @@
 #include "decode.cuh"
 #include "trunk.cuh"
 #include "gdn.cuh"
+#include "rope.cuh"
+#include "kv_cache.cuh"
+#include "paged_attn.cuh"
 #include "quantize.cuh"
 #include "synth.cuh"
 #include "split.inl"
@@ -58,3 +67,6 @@
 #include "trunk.inl"
 #include "gguf.inl"
 #include "gdn.inl"
+#include "rope.inl"
+#include "kv_cache.inl"
+#include "paged_attn.inl"

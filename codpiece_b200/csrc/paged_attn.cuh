@@ -1,0 +1,815 @@
+// paged_attn.cuh — attention over the paged 8-bit cache (kv_cache.cuh): what the
+// kernels share, and the kernel for few query rows (decode).
+//
+// Row (token i, head hq) of a sequence with q_len new tokens and kv_len cached
+// ones (the new ones included) sees the keys j < limit, limit = kv_len - q_len
+// + i + 1 (causal) or kv_len:
+//   z_j = scale * k_scale[page(j)] * <q, kc_j>,  out = sum_j softmax(z)_j v_scale[page(j)] vc_j
+// and lse = log sum_j exp(z_j). A row that sees nothing gives 0 and -inf.
+//
+// Numbers. An int8 or e4m3 code is exact in fp16, so the products run on fp16
+// tensor cores with the page scales applied in fp32 around them. q is brought
+// to fp16 by a power of two per row: one term holds an fp16 or bf16 value
+// exactly; an fp32 value takes two (22 bits, the second the rounding error of
+// the first). Probabilities enter the second product the same way: one fp16
+// term for 16-bit outputs, two for fp32. The softmax reference of a row is
+// kept 8 (in log2) under the running maximum and moves when a score exceeds it
+// by more than 11, so probabilities lie in [0, 2^11] and small ones keep their
+// bits; a page's v_scale enters as its ratio to a reference scale, which moves
+// when a ratio exceeds 8. Sums are fp32.
+//
+// Work. The query rows of one kv head and sequence, (token, head of the group)
+// in that order, form row tiles of kRows rows; a unit is (sequence, row tile,
+// kv head) with its visible keys in tiles. All units' tiles in a row form one
+// range that is cut into equal shares, one per CTA: ragged batches, causal
+// triangles and one long sequence balance alike. A unit that is cut leaves
+// partial sums, softmax reference and row sums in the workspace, which
+// attn_combine_kernel joins in key order (same split, same result).
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+#include "gemm_tc.cuh"   // TMA and mbarrier helpers
+#include "kv_cache.cuh"
+
+namespace cpq {
+
+constexpr int kAttnMaxSeqs = 1024;
+
+struct alignas(64) AttnArgs {
+    CUtensorMap tmap_k, tmap_v;  // codes as [n_pages * n_head_kv * block][D] bytes, box 128 x min(block, 32)
+    const uint8_t *k, *v;
+    const float *k_scale, *v_scale;
+    int64_t n_pages;
+    int block, hkv;
+    const void *q;
+    int64_t qs_tok, qs_head;     // elements
+    void *out;
+    int64_t os_tok, os_head;
+    float *lse;                  // [t][hkv * group], or null
+    int type;                    // of q and out
+    int t, group, n_seqs;
+    const int32_t *seq_start, *kv_len, *table;
+    int64_t table_stride;
+    int max_blocks, causal;
+    float scale_log2;            // softmax scale * log2(e)
+    int min_tiles;               // a CTA's share is at least this many tiles
+    // workspace: two slots per CTA (the unit that ends in it, the unit that begins in it)
+    float *part_o;               // [slot][kRows][D]
+    float2 *part_ml;             // [slot][kRows]: softmax reference, row sum
+    int4 *part_hdr;              // [slot]: sequence, row tile, kv head, 0 unused | 1 goes on | 2 the unit's end
+};
+
+// ---- the split ------------------------------------------------------------------
+
+struct AttnSeq {
+    int row0, q, kv;  // first token, tokens, keys
+};
+
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int s) {
+    AttnSeq r;
+    r.row0 = min(max(a.seq_start[s], 0), a.t);
+    r.q = min(max(a.seq_start[s + 1], r.row0), a.t) - r.row0;
+    r.kv = int(min(int64_t(max(a.kv_len[s], 0)), int64_t(a.max_blocks) * a.block));
+    return r;
+}
+
+// Keys that the rows [r * rows, (r + 1) * rows) see together.
+__device__ __forceinline__ int attn_kv_end(const AttnSeq &s, int r, int rows, int group, int causal) {
+    if (!causal) return s.kv;
+    const int last = (min(s.q * group, (r + 1) * rows) - 1) / group;
+    return min(max(s.kv - s.q + last + 1, 0), s.kv);
+}
+
+__device__ __forceinline__ int attn_row_tiles(const AttnSeq &s, int rows, int group) { return (s.q * group + rows - 1) / rows; }
+
+// A CTA's share of the tiles, and the units in it in order.
+struct AttnPlan {
+    AttnSeq seq[kAttnMaxSeqs];
+    int through[kAttnMaxSeqs + 1];  // tiles before each sequence
+    int s, r, h, tile, left;        // where this CTA begins, and its tiles
+    int n_cta;                      // CTAs that have a share
+};
+
+// Fills the plan (all threads of the CTA; two barriers inside). A unit with no
+// visible key counts one tile, so that some CTA writes its rows.
+template <int ROWS, int TILE>
+__device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
+    auto tiles = [&](const AttnSeq &s, int r) {
+        return max(1, (attn_kv_end(s, r, ROWS, a.group, a.causal) + TILE - 1) / TILE);
+    };
+    for (int s = tid; s < a.n_seqs; s += blockDim.x) {
+        const AttnSeq q = attn_seq(a, s);
+        p.seq[s] = q;
+        const int n = attn_row_tiles(q, ROWS, a.group);
+        int w = -1;  // many row tiles: counted by a warp below
+        if (n <= 4) {
+            w = 0;
+            for (int r = 0; r < n; r++) w += tiles(q, r);
+        }
+        p.through[s + 1] = w < 0 ? -1 : w * a.hkv;
+    }
+    __syncthreads();
+    for (int s = warp; s < a.n_seqs; s += n_warps) {
+        if (p.through[s + 1] >= 0) continue;
+        const AttnSeq q = p.seq[s];
+        const int n = attn_row_tiles(q, ROWS, a.group);
+        int w = 0;
+        for (int r = lane; r < n; r += 32) w += tiles(q, r);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        __syncwarp();
+        if (lane == 0) p.through[s + 1] = w * a.hkv;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
+            int w = s0 + lane < a.n_seqs ? p.through[s0 + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, w, o);
+                if (lane >= o) w += u;
+            }
+            if (s0 + lane < a.n_seqs) p.through[s0 + lane + 1] = sum + w;
+            sum += __shfl_sync(0xffffffffu, w, 31);
+        }
+        if (lane == 0) p.through[0] = 0;
+        __syncwarp();
+        const int n_cta = max(1, min(int(gridDim.x), sum / a.min_tiles));
+        const int c = blockIdx.x;
+        const int x0 = c < n_cta ? int(int64_t(sum) * c / n_cta) : sum;
+        const int x1 = c < n_cta ? int(int64_t(sum) * (c + 1) / n_cta) : sum;
+        int s = 0, r = 0, h = 0, tile = 0;
+        if (x1 > x0) {
+            int lo = 0, hi = a.n_seqs;  // the last sequence that begins at or before x0 and has tiles there
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (p.through[mid] <= x0) lo = mid;
+                else hi = mid;
+            }
+            s = lo;
+            int rem = x0 - p.through[s];
+            const AttnSeq q = p.seq[s];
+            const int n = attn_row_tiles(q, ROWS, a.group);
+            for (int r0 = 0; r0 < n; r0 += 32) {  // row tiles in order, each with its hkv units
+                const int mine = r0 + lane < n ? tiles(q, r0 + lane) * a.hkv : 0;
+                int w = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, w, o);
+                    if (lane >= o) w += u;
+                }
+                const unsigned after = __ballot_sync(0xffffffffu, w > rem);
+                if (after) {
+                    const int at = __ffs(int(after)) - 1;
+                    const int before = __shfl_sync(0xffffffffu, w - mine, at);
+                    const int per = __shfl_sync(0xffffffffu, mine, at) / a.hkv;
+                    r = r0 + at;
+                    h = (rem - before) / per;
+                    tile = (rem - before) - h * per;
+                    break;
+                }
+                rem -= __shfl_sync(0xffffffffu, w, 31);
+            }
+        }
+        if (lane == 0) p.s = s, p.r = r, p.h = h, p.tile = tile, p.left = x1 - x0, p.n_cta = n_cta;
+    }
+    __syncthreads();
+}
+
+// One unit's part in this CTA.
+struct AttnUnit {
+    int s, r, h;
+    AttnSeq seq;
+    int kv_end, t0, t1, n;  // keys seen, tiles [t0, t1) of n here
+};
+
+// Walks the CTA's units; every role of the CTA does so by itself.
+template <int ROWS, int TILE>
+struct AttnWalk {
+    const AttnArgs &a;
+    const AttnPlan &p;
+    int s, r, h, tile, left;
+    __device__ AttnWalk(const AttnArgs &a_, const AttnPlan &p_) : a(a_), p(p_), s(p_.s), r(p_.r), h(p_.h), tile(p_.tile), left(p_.left) {}
+    __device__ bool next(AttnUnit &u) {
+        if (left <= 0) return false;
+        u.s = s, u.r = r, u.h = h;
+        u.seq = p.seq[s];
+        u.kv_end = attn_kv_end(u.seq, r, ROWS, a.group, a.causal);
+        u.n = max(1, (u.kv_end + TILE - 1) / TILE);
+        u.t0 = tile;
+        u.t1 = min(u.n, tile + left);
+        left -= u.t1 - u.t0;
+        tile = 0;
+        if (++h == a.hkv) {
+            h = 0;
+            if (++r == attn_row_tiles(u.seq, ROWS, a.group)) {
+                r = 0;
+                do s++;
+                while (s < a.n_seqs && p.seq[s].q == 0);
+            }
+        }
+        return true;
+    }
+};
+
+// The workspace slot of a cut unit: 0 when it began in an earlier CTA, 1 when it begins here.
+__device__ __forceinline__ int attn_slot(const AttnUnit &u) { return 2 * int(blockIdx.x) + (u.t0 == 0 ? 1 : 0); }
+
+// Marks both of this CTA's slots unused, before any is written.
+__device__ __forceinline__ void attn_clear_slots(const AttnArgs &a) {
+    a.part_hdr[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    a.part_hdr[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
+}
+
+// The page of a sequence's block b, or -1 when it is no page of the pool (its
+// keys then count as absent).
+__device__ __forceinline__ int attn_page(const AttnArgs &a, int s, int b) {
+    if (b >= a.max_blocks) return -1;
+    const int page = a.table[int64_t(s) * a.table_stride + b];
+    return page >= 0 && int64_t(page) < a.n_pages ? page : -1;
+}
+
+__device__ __forceinline__ float attn_q_at(const AttnArgs &a, int64_t i) {
+    if (a.type == CPQ_TYPE_F32) return static_cast<const float *>(a.q)[i];
+    if (a.type == CPQ_TYPE_F16) return __half2float(static_cast<const __half *>(a.q)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(a.q)[i]);
+}
+
+__device__ __forceinline__ void attn_out_at(const AttnArgs &a, int64_t i, float v) {
+    if (a.type == CPQ_TYPE_F32) static_cast<float *>(a.out)[i] = v;
+    else if (a.type == CPQ_TYPE_F16) static_cast<__half *>(a.out)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16 *>(a.out)[i] = __float2bfloat16_rn(v);
+}
+
+// 1 / sum of a row; a row that sees nothing has sum 0 and stays 0, NaN stays NaN.
+__device__ __forceinline__ float attn_inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+
+// The power of two that brings a row's largest magnitude into [2^13, 2^14), as an exponent.
+__device__ __forceinline__ int attn_q_shift(float amax) {
+    const int e = int(__float_as_uint(amax) >> 23) - 127;  // amax >= 0; zero and subnormal: -127
+    if (e == 128) return 0;                                // infinity or NaN: left as it is
+    return 13 - max(e, -100);
+}
+__device__ __forceinline__ float attn_exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr float kAttnRefDrop = 8.0f;    // the reference lies this far under the maximum it was set by
+constexpr float kAttnRefMove = 11.0f;   // and moves when a score is this far above it
+constexpr float kAttnVRatio = 8.0f;     // the v_scale reference moves when a page's scale is this many times it
+constexpr float kLn2 = 0.69314718055994531f;
+
+// lse of a row from its reference (log2) and sum.
+__device__ __forceinline__ float attn_lse(float ref, float sum) {
+    return sum == 0.0f ? __int_as_float(0xff800000) : (ref + __log2f(sum)) * kLn2;
+}
+
+// ---- few query rows: mma.sync tiles, one key tile per warp -------------------------
+//
+// Decode reads the cache once and does little with it, so the kernel is built
+// around the copy: one CTA per SM, a producer warp that keeps a ring of 32-key
+// tiles (K and V codes, TMA boxes of 128 bytes x up to 32 keys, 128-byte
+// swizzle) in flight, and eight warps that each take every eighth tile with
+// their own softmax state and output accumulators, so that nothing but the
+// end of a unit makes warps wait for one another. m16n8k16 fp16 MMAs: 16 rows
+// of 16-bit q, or 8 rows of fp32 q with the first terms in rows 0-7 and the
+// second terms in rows 8-15 of the same MMA (they meet in one thread, lanes
+// of row g hold both), so fp32 costs no extra MMA.
+//
+// Operand order. A key tile's codes go from shared memory to the MMA's B
+// registers without a transpose:
+//   K: lane (g, t) takes chunks 2t, 2t + 1 (16 bytes each) of key g's 128-byte
+//      half row: 32 dims 32 t + 4 j + i, MMA j of 8 taking i = 0..3 as k =
+//      2t, 2t + 1, 2t + 8, 2t + 9 (q is stored in that order).
+//   V: lane (g, t) takes chunk g of keys 2t, 2t + 1, 2t + 8, 2t + 9: n-tile b
+//      of 16 then has column n = dim 16 n + b, its k the four keys, paired
+//      from two keys' words by byte permutes.
+// With the 128-byte swizzle (chunk ^ (key & 7)) each quarter warp's 16-byte
+// loads touch eight different bank groups in both.
+
+constexpr int kAttnTile = 32;
+constexpr int kAttnWarps = 8;
+constexpr int kAttnThreads = 32 * (kAttnWarps + 1);
+
+template <int D, bool SPLIT> struct DecCfg {
+    static constexpr int kRows = SPLIT ? 8 : 16;
+    static constexpr int kHalfBytes = kAttnTile * D;              // K or V codes of a tile
+    static constexpr int kStageBytes = 2 * kHalfBytes;
+    static constexpr int kStages = D == 256 ? (SPLIT ? 10 : 8) : (SPLIT ? 20 : 18);
+    static constexpr int kRedBytes = 4 * kRows * D * 4;          // four warps' accumulators
+    static constexpr int kQBytes = D / 16 * 512;
+    static constexpr int kQOff = kStages * kStageBytes;
+    static constexpr int kRedOff = kQOff + kQBytes;
+    static constexpr int kSmallOff = kRedOff + kRedBytes;
+    // small: stage info float4, full/empty barriers, stats (ref, sum, v reference) per warp and row, row factors
+    static constexpr int kInfoOff = kSmallOff;
+    static constexpr int kBarOff = kInfoOff + kStages * 16;
+    static constexpr int kStatOff = kBarOff + kStages * 16;
+    static constexpr int kRowOff = kStatOff + kAttnWarps * 16 * 8 + kAttnWarps * 16;
+    static constexpr int kPlanOff = (kRowOff + 16 * 16 + 127) / 128 * 128;
+    static constexpr int kSmem = kPlanOff + int(sizeof(AttnPlan)) + 1024;
+};
+static_assert(DecCfg<256, true>::kSmem <= 227 * 1024 && DecCfg<256, false>::kSmem <= 227 * 1024 &&
+                  DecCfg<128, true>::kSmem <= 227 * 1024 && DecCfg<128, false>::kSmem <= 227 * 1024,
+              "shared memory");
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Codes (bytes 0, 1) and (bytes 2, 3) of w as fp16 pairs, exact. int8: 0x6400 |
+// (code + 128) is 1152 + code.
+template <int FMT>
+__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if constexpr (FMT == CPQ_KV_INT8) {
+        w ^= 0x80808080u;
+        const __half2 k1152 = __float2half2_rn(1152.0f);
+        lo = h2u(__hsub2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), k1152));
+        hi = h2u(__hsub2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), k1152));
+    } else {
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float a, float b) { return h2u(__floats2half2_rn(a, b)); }
+
+__device__ __forceinline__ void dec_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kAttnWarps) : "memory"); }
+
+template <int D, int FMT, bool SPLIT>
+__global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __grid_constant__ AttnArgs a) {
+    using C = DecCfg<D, SPLIT>;
+    constexpr int kRows = C::kRows, NA = D / 128;  // 128-byte atoms per key
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint4 *sq = reinterpret_cast<uint4 *>(smem + C::kQOff);
+    float *red = reinterpret_cast<float *>(smem + C::kRedOff);
+    float4 *info = reinterpret_cast<float4 *>(smem + C::kInfoOff);  // k_scale, v_scale of keys 0-15 and 16-31 (NaN: no page)
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff), *empty = full + C::kStages;
+    float2 *stat = reinterpret_cast<float2 *>(smem + C::kStatOff);  // [warp][16 rows]: reference, sum
+    float *vstat = reinterpret_cast<float *>(stat + kAttnWarps * 16);
+    float *rowf = reinterpret_cast<float *>(smem + C::kRowOff);     // [row]: 2^-shift of its q
+    AttnPlan &plan = *reinterpret_cast<AttnPlan *>(smem + C::kPlanOff);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        fence_mbar_init();
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    attn_make_plan<kRows, kAttnTile>(a, plan);
+    if (threadIdx.x == 0) attn_clear_slots(a);
+    AttnWalk<kRows, kAttnTile> walk(a, plan);
+    AttnUnit u;
+    const int lb = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
+
+    if (warp == kAttnWarps) {
+        // ---- producer: 32 tiles' pages and scales at a time, one tile per lane ----
+        const int pages = a.block == 16 ? 2 : 1, box = a.block < kAttnTile ? a.block : kAttnTile;
+        int g = 0;  // tiles issued
+        bool ok = true;
+        while (ok && walk.next(u)) {
+            for (int b0 = u.t0; b0 < u.t1 && ok; b0 += 32) {
+                int page[2] = {-1, -1};
+                float ks[2], vs[2];
+                const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    ks[j] = vs[j] = nan;
+                    const int key = (b0 + lane) * kAttnTile + 16 * j;
+                    if (b0 + lane < u.t1 && key < u.kv_end && j < pages) page[j] = attn_page(a, u.s, key >> lb);
+                    if (page[j] >= 0) {
+                        ks[j] = a.k_scale[int64_t(page[j]) * a.hkv + u.h];
+                        vs[j] = a.v_scale[int64_t(page[j]) * a.hkv + u.h];
+                    }
+                }
+                if (pages == 1) ks[1] = ks[0], vs[1] = vs[0];
+                const int n = min(32, u.t1 - b0);
+                for (int i = 0; i < n; i++, g++) {
+                    const int st = g % C::kStages;
+                    const float4 f = make_float4(__shfl_sync(0xffffffffu, ks[0], i), __shfl_sync(0xffffffffu, vs[0], i),
+                                                 __shfl_sync(0xffffffffu, ks[1], i), __shfl_sync(0xffffffffu, vs[1], i));
+                    const int p0 = __shfl_sync(0xffffffffu, page[0], i), p1 = __shfl_sync(0xffffffffu, page[1], i);
+                    if (lane == 0) ok = mbar_wait_bounded(&empty[st], (uint32_t(g / C::kStages) & 1u) ^ 1u);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                    if (!ok) break;
+                    if (lane == 0) {
+                        info[st] = f;
+                        const int have = (p0 >= 0) + (p1 >= 0);
+                        mbar_arrive_expect_tx(&full[st], uint32_t(have * box) * (2u * D));
+                        uint8_t *dst = smem + st * C::kStageBytes;
+                        for (int j = 0; j < pages; j++) {
+                            const int pg = j ? p1 : p0;
+                            if (pg < 0) continue;
+                            // the tile's first key inside its page
+                            const int in = j ? 0 : ((b0 + i) * kAttnTile) & (a.block - 1);
+                            const int row = (pg * a.hkv + u.h) * a.block + in;
+#pragma unroll
+                            for (int at = 0; at < NA; at++) {
+                                tma_load_2d(dst + at * (kAttnTile * 128) + j * (16 * 128), &a.tmap_k, at * 128, row, &full[st]);
+                                tma_load_2d(dst + C::kHalfBytes + at * (kAttnTile * 128) + j * (16 * 128), &a.tmap_v, at * 128, row,
+                                            &full[st]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        // no copy may land after the CTA has left
+        if (lane == 0)
+            for (int x = g > C::kStages ? g - C::kStages : 0; x < g; x++)
+                mbar_wait_bounded(&full[x % C::kStages], uint32_t(x / C::kStages) & 1u);
+        return;
+    }
+
+    // ---- eight warps: tile x of the CTA goes to warp x % 8 ----
+    const int gq = lane >> 2, tq = lane & 3;
+    int base = 0;       // tiles of the units before
+    bool dead = false;  // a wait has given up: take part in barriers only
+    while (walk.next(u)) {
+        // q of the unit's rows, as A fragments in the K order above
+        for (int rr = warp; rr < kRows; rr += kAttnWarps) {
+            const int row = u.r * kRows + rr;
+            const bool there = row < u.seq.q * a.group;
+            constexpr int E = D / 32;
+            float x[E], m = 0.0f;
+            const int tok = u.seq.row0 + row / a.group, head = u.h * a.group + row % a.group;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                x[e] = there ? attn_q_at(a, tok * a.qs_tok + head * a.qs_head + lane * E + e) : 0.0f;
+                m = fmaxf(m, fabsf(x[e]));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int sh = attn_q_shift(m);
+            if (lane == 0) rowf[rr] = attn_exp2i(-sh);
+            const float f = attn_exp2i(sh);
+#pragma unroll
+            for (int e = 0; e < E; e += 4) {
+                const int d = lane * E + e;  // a group of four dims: one MMA's share of lane t
+                uint32_t *to = reinterpret_cast<uint32_t *>(sq + ((d >> 7) * 8 + ((d >> 2) & 7)) * 32 + (rr & 7) * 4 + ((d >> 5) & 3));
+                float hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    hi[k] = __half2float(__float2half_rn(x[e + k] * f));
+                    lo[k] = x[e + k] * f - hi[k];
+                }
+                to[rr >> 3] = pack_h2(hi[0], hi[1]);
+                to[2 + (rr >> 3)] = pack_h2(hi[2], hi[3]);
+                if constexpr (SPLIT) {
+                    to[1] = pack_h2(lo[0], lo[1]);
+                    to[3] = pack_h2(lo[2], lo[3]);
+                }
+            }
+        }
+        dec_sync();
+
+        constexpr int NR = SPLIT ? 1 : 2;  // real rows per lane: gq (and gq + 8)
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        const float ninf = __int_as_float(0xff800000);
+        float ref[NR], sum[NR], qf[NR];
+        int lim[NR];
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            ref[k] = ninf;
+            sum[k] = 0.0f;
+            const int row = u.r * kRows + gq + 8 * k;
+            qf[k] = rowf[gq + 8 * k] * a.scale_log2;
+            lim[k] = a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + row / a.group + 1) : u.seq.kv;
+        }
+        float vref = 0.0f;
+        const int n_here = u.t1 - u.t0;
+        // every tile of the CTA has one warp: tile x of it (counted over units) goes to warp x % 8
+        for (int x = (warp - base % kAttnWarps + kAttnWarps) % kAttnWarps; x < n_here; x += kAttnWarps) {
+            const int gx = base + x, st = gx % C::kStages;
+            if (!dead && !mbar_wait_bounded(&full[st], uint32_t(gx / C::kStages) & 1u)) dead = true;
+            dead = __any_sync(0xffffffffu, dead);
+            if (dead) continue;
+            const int key0 = (u.t0 + x) * kAttnTile;
+            const float4 sc = info[st];
+            const uint8_t *sk = smem + st * C::kStageBytes, *sv = sk + C::kHalfBytes;
+            float s[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
+#pragma unroll
+            for (int at = 0; at < NA; at++) {
+                uint4 kw[4][2];
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        kw[nt][c] = *reinterpret_cast<const uint4 *>(sk + at * (kAttnTile * 128) + (8 * nt + gq) * 128 +
+                                                                     (((2 * tq + c) ^ gq) << 4));
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint4 qw = sq[(at * 8 + j) * 32 + lane];
+                    const uint32_t qa[4] = {qw.x, qw.y, qw.z, qw.w};
+#pragma unroll
+                    for (int nt = 0; nt < 4; nt++) {
+                        const uint4 w = kw[nt][j >> 2];
+                        const uint32_t word = (j & 3) == 0 ? w.x : (j & 3) == 1 ? w.y : (j & 3) == 2 ? w.z : w.w;
+                        uint32_t b0, b1;
+                        codes_h2<FMT>(word, b0, b1);
+                        mma_f16(s[nt], qa, b0, b1);
+                    }
+                }
+            }
+            // scores in log2, masked; a page that is not there has NaN scales
+            const bool in0 = sc.x == sc.x, in1 = sc.z == sc.z;
+            float p[NR][8];
+            float mx[NR];
+#pragma unroll
+            for (int k = 0; k < NR; k++) {
+                mx[k] = ninf;
+#pragma unroll
+                for (int nt = 0; nt < 4; nt++) {
+                    const float f = qf[k] * (nt < 2 ? sc.x : sc.z);
+                    const bool in = nt < 2 ? in0 : in1;
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const int key = key0 + 8 * nt + 2 * tq + c;
+                        const float z = SPLIT ? s[nt][c] + s[nt][c + 2] : s[nt][2 * k + c];
+                        p[k][2 * nt + c] = in && key < lim[k] ? z * f : ninf;
+                        mx[k] = fmaxf(mx[k], p[k][2 * nt + c]);
+                    }
+                }
+                mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
+                mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
+            }
+            // references: moved for the whole warp at once, seldom
+            const float vmax = fmaxf(in0 ? sc.y : 0.0f, in1 ? sc.w : 0.0f);
+            bool move = vmax > kAttnVRatio * vref;
+#pragma unroll
+            for (int k = 0; k < NR; k++) move |= mx[k] > ref[k] + kAttnRefMove;
+            if (__any_sync(0xffffffffu, move)) {
+                const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
+                const float vf = vnew > 0.0f ? vref / vnew : 0.0f;
+                vref = vnew;
+                float of[NR];
+#pragma unroll
+                for (int k = 0; k < NR; k++) {
+                    float f = 1.0f;
+                    if (mx[k] > ref[k] + kAttnRefMove) {
+                        const float to = mx[k] - kAttnRefDrop;
+                        f = ex2(ref[k] - to);  // 0 for the first scores (ref = -inf)
+                        ref[k] = to;
+                    }
+                    sum[k] *= f;
+                    of[k] = f * vf;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    o[i][0] *= of[0], o[i][1] *= of[0];
+                    o[i][2] *= of[NR - 1], o[i][3] *= of[NR - 1];
+                }
+            }
+            const float r0 = in0 && vref > 0.0f ? sc.y / vref : 0.0f, r1 = in1 && vref > 0.0f ? sc.w / vref : 0.0f;
+#pragma unroll
+            for (int k = 0; k < NR; k++) {
+                const float base_ref = ref[k] == ninf ? 0.0f : ref[k];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float e = ex2(p[k][i] - base_ref);
+                    sum[k] += e;
+                    p[k][i] = e * (i < 4 ? r0 : r1);
+                }
+            }
+            // O += P V
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                uint32_t pa[4];
+                if constexpr (SPLIT) {
+                    const float *pp = &p[0][4 * ks];
+                    const __half2 h0 = __floats2half2_rn(pp[0], pp[1]), h1 = __floats2half2_rn(pp[2], pp[3]);
+                    pa[0] = h2u(h0);
+                    pa[2] = h2u(h1);
+                    pa[1] = pack_h2(pp[0] - __low2float(h0), pp[1] - __high2float(h0));
+                    pa[3] = pack_h2(pp[2] - __low2float(h1), pp[3] - __high2float(h1));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        pa[k] = pack_h2(p[k][4 * ks], p[k][4 * ks + 1]);
+                        pa[k + 2] = pack_h2(p[k][4 * ks + 2], p[k][4 * ks + 3]);
+                    }
+                }
+                // e4m3: bytes of keys that are not there may be NaN, which 0 * NaN would keep
+                uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+                if constexpr (FMT != CPQ_KV_INT8) {
+                    const bool in = ks ? in1 : in0;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        keep[i] = in && key0 + 16 * ks + 2 * tq + (i & 1) + 8 * (i >> 1) < u.seq.kv ? ~0u : 0u;
+                }
+#pragma unroll
+                for (int at = 0; at < NA; at++) {
+                    uint4 vw[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int key = 16 * ks + 2 * tq + (i & 1) + 8 * (i >> 1);
+                        vw[i] = *reinterpret_cast<const uint4 *>(sv + at * (kAttnTile * 128) + key * 128 + ((gq ^ (key & 7)) << 4));
+                    }
+#pragma unroll
+                    for (int wi = 0; wi < 4; wi++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            w[i] = wi == 0 ? vw[i].x : wi == 1 ? vw[i].y : wi == 2 ? vw[i].z : vw[i].w;
+                            if constexpr (FMT != CPQ_KV_INT8) w[i] &= keep[i];
+                        }
+                        uint32_t b[4][2];
+                        codes_h2<FMT>(__byte_perm(w[0], w[1], 0x5140), b[0][0], b[1][0]);
+                        codes_h2<FMT>(__byte_perm(w[0], w[1], 0x7362), b[2][0], b[3][0]);
+                        codes_h2<FMT>(__byte_perm(w[2], w[3], 0x5140), b[0][1], b[1][1]);
+                        codes_h2<FMT>(__byte_perm(w[2], w[3], 0x7362), b[2][1], b[3][1]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mma_f16(o[at * 16 + wi * 4 + i], pa, b[i][0], b[i][1]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        base += n_here;
+
+        // join the eight warps: stats first, then the accumulators at the common reference
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+            sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+            if (tq == 0) stat[warp * 16 + gq + 8 * k] = make_float2(ref[k], sum[k]);
+        }
+        if (lane == 0) vstat[warp] = vref;
+        dec_sync();
+        float top[NR], all[NR];
+#pragma unroll
+        for (int k = 0; k < NR; k++) {
+            top[k] = ninf;
+            all[k] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; w++) top[k] = fmaxf(top[k], stat[w * 16 + gq + 8 * k].x);
+            const float b = top[k] == ninf ? 0.0f : top[k];
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; w++) {
+                const float2 x = stat[w * 16 + gq + 8 * k];
+                all[k] += x.y * ex2(x.x - b);
+            }
+        }
+        // fragment order: [16 at + b][row][n], dim 128 at + 16 n + b
+        float *mine = red + (warp & 3) * (kRows * D);
+        auto put = [&](bool add) {
+#pragma unroll
+            for (int k = 0; k < NR; k++) {
+                const float f = ex2(ref[k] - (top[k] == ninf ? 0.0f : top[k])) * vref;
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    float2 *to = reinterpret_cast<float2 *>(mine + (i * kRows + gq + 8 * k) * 8 + 2 * tq);
+                    float2 v = SPLIT ? make_float2((o[i][0] + o[i][2]) * f, (o[i][1] + o[i][3]) * f)
+                                     : make_float2(o[i][2 * k] * f, o[i][2 * k + 1] * f);
+                    if (add) {
+                        const float2 w = *to;
+                        v.x += w.x, v.y += w.y;
+                    }
+                    *to = v;
+                }
+            }
+        };
+        if (warp >= 4) put(false);
+        dec_sync();
+        if (warp < 4) put(true);
+        if (warp == 0 && tq == 0) {
+#pragma unroll
+            for (int k = 0; k < NR; k++) stat[gq + 8 * k] = make_float2(top[k], all[k]);
+        }
+        dec_sync();
+        const bool whole = u.t0 == 0 && u.t1 == u.n;
+        const int slot = attn_slot(u);
+        for (int i = threadIdx.x; i < kRows * (D / 16); i += 32 * kAttnWarps) {
+            const int n = i & 7, rr = (i >> 3) % kRows, at = (i >> 3) / kRows;
+            const int row = u.r * kRows + rr;
+            const bool there = row < u.seq.q * a.group;
+            float v[16];
+#pragma unroll
+            for (int b = 0; b < 16; b++) {
+                const int e = ((at * 16 + b) * kRows + rr) * 8 + n;
+                v[b] = (red[e] + red[kRows * D + e]) + (red[2 * kRows * D + e] + red[3 * kRows * D + e]);
+            }
+            const int d0 = at * 128 + n * 16;
+            const float2 ml = stat[rr];
+            if (whole) {
+                if (there) {
+                    const float f = attn_inverse(ml.y);
+                    const int tok = u.seq.row0 + row / a.group, head = u.h * a.group + row % a.group;
+                    const int64_t to = tok * a.os_tok + head * a.os_head + d0;
+#pragma unroll
+                    for (int b = 0; b < 16; b++) attn_out_at(a, to + b, v[b] * f);
+                    if (d0 == 0 && a.lse) a.lse[int64_t(tok) * (a.hkv * a.group) + head] = attn_lse(ml.x, ml.y);
+                }
+            } else {
+                float4 *to = reinterpret_cast<float4 *>(a.part_o + (int64_t(slot) * kRows + rr) * D + d0);
+#pragma unroll
+                for (int b = 0; b < 4; b++) to[b] = make_float4(v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]);
+                if (d0 == 0) a.part_ml[slot * kRows + rr] = ml;
+                if (i == 0) a.part_hdr[slot] = make_int4(u.s, u.r, u.h, u.t1 == u.n ? 2 : 1);
+            }
+        }
+        // q, stats and sums are rewritten by the next unit only after everyone is done with them
+        dec_sync();
+    }
+}
+
+// ---- joining a cut unit ------------------------------------------------------------
+//
+// grid (CTAs of the attention grid, rows): block (c, rr) joins row rr of the
+// unit that begins in CTA c and goes on in c + 1, ...: sum over the parts of
+// part * 2^(reference - largest reference). D / 4 threads across, the parts
+// dealt out over the rest of the block and added in a fixed order.
+
+constexpr int kCombineThreads = 256;
+
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kCombineThreads) attn_combine_kernel(const __grid_constant__ AttnArgs a) {
+    constexpr int kAcross = D / 4, kDeal = kCombineThreads / kAcross;
+    __shared__ float4 s_o[kDeal][kAcross];
+    __shared__ float s_l[kDeal];
+    const int c = blockIdx.x, rr = blockIdx.y;
+    const int x = threadIdx.x % kAcross, z = threadIdx.x / kAcross;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int4 hdr = a.part_hdr[2 * c + 1];
+    if (hdr.w == 0) return;
+    const AttnSeq seq = attn_seq(a, hdr.x);
+    const int row = hdr.y * ROWS + rr;
+    if (row >= seq.q * a.group) return;
+    // parts: slot 2c + 1, then 2(c + 1), 2(c + 2), ... up to the one that ends the unit
+    __shared__ int s_n;
+    if (threadIdx.x == 0) s_n = int(gridDim.x) - c;
+    __syncthreads();
+    for (int i = threadIdx.x; i < int(gridDim.x) - c; i += kCombineThreads) {
+        const int w = i == 0 ? hdr.w : a.part_hdr[2 * (c + i)].w;
+        if (w != 1) atomicMin(&s_n, i + 1);
+    }
+    __syncthreads();
+    const int n = s_n;
+    auto slot = [&](int i) { return int64_t(i == 0 ? 2 * c + 1 : 2 * (c + i)); };
+    __shared__ float s_m[kCombineThreads / 32];
+    float m = __int_as_float(0xff800000);
+    for (int i = threadIdx.x; i < n; i += kCombineThreads) m = fmaxf(m, a.part_ml[slot(i) * ROWS + rr].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kCombineThreads / 32; w++) m = fmaxf(m, s_m[w]);
+    const float b = m == __int_as_float(0xff800000) ? 0.0f : m;
+    float4 acc = make_float4(0, 0, 0, 0);
+    float l = 0.0f;
+#pragma unroll 4
+    for (int i = z; i < n; i += kDeal) {
+        const float2 ml = a.part_ml[slot(i) * ROWS + rr];
+        const float4 v = *reinterpret_cast<const float4 *>(a.part_o + (slot(i) * ROWS + rr) * D + 4 * x);
+        const float f = ex2(ml.x - b);
+        acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
+        l += ml.y * f;
+    }
+    s_o[z][x] = acc;
+    if (x == 0) s_l[z] = l;
+    __syncthreads();
+    if (z) return;
+    l = 0.0f;
+    acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < kDeal; i++) {
+        const float4 v = s_o[i][x];
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        l += s_l[i];
+    }
+    const float f = attn_inverse(l);
+    const int tok = seq.row0 + row / a.group, head = hdr.z * a.group + row % a.group;
+    const int64_t to = tok * a.os_tok + head * a.os_head + 4 * x;
+    attn_out_at(a, to, acc.x * f);
+    attn_out_at(a, to + 1, acc.y * f);
+    attn_out_at(a, to + 2, acc.z * f);
+    attn_out_at(a, to + 3, acc.w * f);
+    if (x == 0 && a.lse) a.lse[int64_t(tok) * (a.hkv * a.group) + head] = attn_lse(m, l);
+}
+
+}  // namespace cpq

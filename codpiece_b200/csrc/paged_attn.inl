@@ -1,0 +1,138 @@
+// paged_attn.inl — cpq_paged_attn: host side of paged_attn.cuh.
+
+namespace cpq {
+
+// The cache's codes as a byte matrix of head rows, box 128 bytes x up to 32 keys, 128-byte swizzle.
+static cpq_status kv_tensor_map(const cpq_kv_cache *c, const void *codes, CUtensorMap *out) {
+    EncodeTiledFn enc = encode_tiled();
+    if (!enc) return fail(CPQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[2] = {cuuint64_t(c->head_dim), cuuint64_t(c->n_pages) * cuuint64_t(c->n_head_kv) * cuuint64_t(c->block)};
+    const cuuint64_t strides[1] = {cuuint64_t(c->head_dim)};
+    const cuuint32_t box[2] = {128, cuuint32_t(std::min(c->block, kAttnTile))};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr,
+                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? CPQ_SUCCESS : fail(CPQ_ERR_CUDA, "cuTensorMapEncodeTiled (kv cache) failed (%d)", int(r));
+}
+
+// Workspace of a launch of `ctas` CTAs with `rows` rows per unit: partial accumulators, statistics, headers.
+static size_t attn_ws_bytes(int ctas, int rows, int d) {
+    const size_t slots = 2 * size_t(ctas);
+    return align_up(slots * rows * d * 4, 256) + align_up(slots * rows * 8, 256) + align_up(slots * 16, 256);
+}
+
+static void attn_carve(AttnArgs &a, void *ws, int ctas, int rows, int d) {
+    const size_t slots = 2 * size_t(ctas);
+    uint8_t *p = static_cast<uint8_t *>(ws);
+    a.part_o = reinterpret_cast<float *>(p);
+    p += align_up(slots * rows * d * 4, 256);
+    a.part_ml = reinterpret_cast<float2 *>(p);
+    p += align_up(slots * rows * 8, 256);
+    a.part_hdr = reinterpret_cast<int4 *>(p);
+}
+
+template <int D, int FMT, bool SPLIT>
+static cudaError_t launch_attn_decode(const AttnArgs &a, int ctas, cudaStream_t st) {
+    using C = DecCfg<D, SPLIT>;
+    static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
+    const int dev = std::max(current_device(), 0);
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (!(set.load() & bit)) {
+        const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, FMT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        if (e != cudaSuccess) return e;
+        set.fetch_or(bit);
+    }
+    cudaError_t e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kAttnThreads), C::kSmem, st, a);
+    if (e != cudaSuccess) return e;
+    return launch(attn_combine_kernel<D, C::kRows>, dim3(unsigned(ctas), unsigned(C::kRows)), dim3(kCombineThreads), 0, st, a);
+}
+
+template <int D, bool SPLIT>
+static cudaError_t launch_attn_fmt(const AttnArgs &a, int fmt, int ctas, cudaStream_t st) {
+    return fmt == CPQ_KV_INT8 ? launch_attn_decode<D, CPQ_KV_INT8, SPLIT>(a, ctas, st)
+                              : launch_attn_decode<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st);
+}
+
+}  // namespace cpq
+
+extern "C" size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *c, const cpq_tensor *q) {
+    using namespace cpq;
+    if (!c || !q) return 0;
+    return attn_ws_bytes(sm_count(std::max(current_device(), 0)), 16, c->head_dim);
+}
+
+extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c, const cpq_attn_seqs *s, float scale,
+                                     int32_t causal, cpq_tensor *out, float *lse, void *workspace, size_t workspace_bytes,
+                                     void *stream) {
+    using namespace cpq;
+    cpq_status st = check_cache(c, "paged_attn");
+    if (st != CPQ_SUCCESS) return st;
+    if (!head_rows(q) || !head_rows(out))
+        return fail(CPQ_ERR_INVALID_ARG, "paged_attn: q and out must be F32, F16 or BF16 with ne=[D, heads, tokens, 1] and contiguous rows");
+    if (q->type != out->type || q->ne[0] != out->ne[0] || q->ne[1] != out->ne[1] || q->ne[2] != out->ne[2])
+        return fail(CPQ_ERR_INVALID_ARG, "paged_attn: out differs from q in type or shape");
+    if (q->ne[0] != c->head_dim || q->ne[1] % c->n_head_kv)
+        return fail(CPQ_ERR_INVALID_ARG, "paged_attn: q ne=[%lld, %lld] does not fit %d kv heads of %d", (long long)q->ne[0],
+                    (long long)q->ne[1], c->n_head_kv, c->head_dim);
+    if (!s) return fail(CPQ_ERR_INVALID_ARG, "paged_attn: null sequences");
+    if (s->n_seqs < 0 || s->max_blocks < 0 || s->table_stride < s->max_blocks)
+        return fail(CPQ_ERR_INVALID_ARG, "paged_attn: n_seqs=%lld max_blocks=%d table stride %lld", (long long)s->n_seqs, s->max_blocks,
+                    (long long)s->table_stride);
+    if (s->n_seqs > kAttnMaxSeqs) return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: %lld sequences (at most %d)", (long long)s->n_seqs, kAttnMaxSeqs);
+    if (!std::isfinite(scale)) return fail(CPQ_ERR_INVALID_ARG, "paged_attn: scale %g", scale);
+    if (q->ne[2] == 0 || s->n_seqs == 0) return CPQ_SUCCESS;
+    if (!s->seq_start || !s->kv_len || (!s->table && s->max_blocks > 0)) return fail(CPQ_ERR_INVALID_ARG, "paged_attn: null sequence pointer");
+    const int64_t rows = q->ne[2] * q->ne[1];
+    if (rows > 2147483647 || c->n_pages * c->n_head_kv * c->block > 2147483647 || int64_t(s->max_blocks) * c->block > 2147483647)
+        return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: more than 2^31 - 1 rows, cache rows or keys");
+    const bool split = q->type == CPQ_TYPE_F32;
+    const int unit_rows = split ? 8 : 16;
+    // the units' tiles are counted in 32 bits
+    const int64_t tiles = std::max<int64_t>(1, (int64_t(s->max_blocks) * c->block + kAttnTile - 1) / kAttnTile);
+    if ((rows / unit_rows + s->n_seqs * c->n_head_kv) > 2147483647 / tiles)
+        return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: %lld rows over up to %lld keys are too many for one call", (long long)rows,
+                    (long long)s->max_blocks * c->block);
+    if (!workspace) return fail(CPQ_ERR_NOT_INITIALIZED, "paged_attn: no workspace");
+    const int ctas = sm_count(std::max(current_device(), 0));
+    if (!aligned(workspace, 256) || workspace_bytes < attn_ws_bytes(ctas, unit_rows, c->head_dim))
+        return fail(CPQ_ERR_WORKSPACE, "paged_attn: workspace of %zu bytes, 256-byte aligned, needs %zu", workspace_bytes,
+                    attn_ws_bytes(ctas, unit_rows, c->head_dim));
+    AttnArgs a{};
+    st = kv_tensor_map(c, c->k, &a.tmap_k);
+    if (st == CPQ_SUCCESS) st = kv_tensor_map(c, c->v, &a.tmap_v);
+    if (st != CPQ_SUCCESS) return st;
+    a.k = static_cast<const uint8_t *>(c->k);
+    a.v = static_cast<const uint8_t *>(c->v);
+    a.k_scale = c->k_scale;
+    a.v_scale = c->v_scale;
+    a.n_pages = c->n_pages;
+    a.block = c->block;
+    a.hkv = c->n_head_kv;
+    const size_t b = size_t(act_bytes(q->type));
+    a.q = q->data;
+    a.qs_head = int64_t(q->nb[1] / b);
+    a.qs_tok = int64_t(q->nb[2] / b);
+    a.out = out->data;
+    a.os_head = int64_t(out->nb[1] / b);
+    a.os_tok = int64_t(out->nb[2] / b);
+    a.lse = lse;
+    a.type = q->type;
+    a.t = int(q->ne[2]);
+    a.group = int(q->ne[1] / c->n_head_kv);
+    a.n_seqs = int(s->n_seqs);
+    a.seq_start = s->seq_start;
+    a.kv_len = s->kv_len;
+    a.table = s->table;
+    a.table_stride = s->table_stride;
+    a.max_blocks = s->max_blocks;
+    a.causal = causal ? 1 : 0;
+    a.scale_log2 = float(double(scale) * 1.4426950408889634);
+    a.min_tiles = kAttnWarps;
+    attn_carve(a, workspace, ctas, unit_rows, c->head_dim);
+    const cudaStream_t cs = static_cast<cudaStream_t>(stream);
+    cudaError_t e;
+    if (c->head_dim == 256) e = split ? launch_attn_fmt<256, true>(a, c->format, ctas, cs) : launch_attn_fmt<256, false>(a, c->format, ctas, cs);
+    else e = split ? launch_attn_fmt<128, true>(a, c->format, ctas, cs) : launch_attn_fmt<128, false>(a, c->format, ctas, cs);
+    return e == cudaSuccess ? CPQ_SUCCESS : cuda_fail(e, "paged_attn launch");
+}

@@ -41,6 +41,7 @@ typedef enum {
     CPQ_TYPE_Q4_K = 12,
     CPQ_TYPE_Q6_K = 14,
     CPQ_TYPE_Q8_K = 15,
+    CPQ_TYPE_BF16 = 30,
 } cpq_type;
 
 /* Status codes. 0 matches GGML_STATUS_SUCCESS; a non-zero status is what the
@@ -397,6 +398,145 @@ void cpq_trunk_destroy(cpq_trunk *trunk);
 cpq_status cpq_gated_delta_net(const cpq_tensor *q, const cpq_tensor *k, const cpq_tensor *v, const cpq_tensor *g,
                                const cpq_tensor *beta, const cpq_tensor *state, cpq_tensor *dst, int32_t n_snap,
                                float *cache, int64_t cache_slot_stride, void *stream);
+
+/* ---- the attention core: rotary positions, paged 8-bit cache, attention ------
+ *
+ * What stands between the q/k/v projections and attn_output in an attention
+ * layer (qwen35.rs:3000-3197: ggml_rope_multi, the cache writes,
+ * ggml_flash_attn_ext), for many requests of different lengths whose keys and
+ * values live in pages of one pool. A step is cpq_kv_slots once, then per
+ * layer cpq_rope_apply on q and k, cpq_kv_append, cpq_paged_attn. Lengths,
+ * tables and slots stay on the device, so a step can be captured in a CUDA
+ * graph. q, k, v and outputs are tensors ne = [D, heads, tokens, 1], F32, F16
+ * or BF16, rows (ne[0]) contiguous, nb[1] and nb[2] any whole number of
+ * elements: views into a projection's output as they are. */
+
+/* Rotary positions with ggml_rope_ext's parameters. */
+typedef enum {
+    CPQ_ROPE_INTERLEAVED = 0, /* pairs (2i, 2i + 1) */
+    CPQ_ROPE_HALF = 1,        /* pairs (i, i + n_dims / 2) */
+} cpq_rope_mode;
+
+typedef struct cpq_rope_params {
+    int32_t n_dims;             /* rotated elements of a head, even, at most 256; the rest is copied */
+    int32_t mode;
+    double base;                /* pair i turns by pos * base^(-2 i / n_dims) */
+    double freq_scale;          /* 1 / context factor: 1, or 1 / s for linear scaling and YaRN */
+    double ext_factor;          /* 0: freq_scale alone; 1: YaRN */
+    double attn_factor;         /* magnitude of the rotated values */
+    double beta_fast, beta_slow; /* YaRN: turns within n_ctx_orig above / below which a pair keeps / loses its frequency */
+    int64_t n_ctx_orig;         /* YaRN: context the model was trained on */
+    const double *freq_factors; /* n_dims / 2 divisors of the frequencies, or NULL */
+} cpq_rope_params;
+
+typedef struct cpq_rope cpq_rope;
+
+/* Frequencies of one model (host memory only). */
+cpq_status cpq_rope_create(const cpq_rope_params *params, cpq_rope **rope);
+void cpq_rope_destroy(cpq_rope *rope);
+/* y[i] = x[i] rotated to positions pos[token] (any int32), for n <= 4 tensors
+ * of one type, head size and token count (q and k together). y[i] may be x[i]
+ * itself (same data and strides); otherwise the two must not overlap. */
+cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *const *x, cpq_tensor *const *y, int n,
+                          const int32_t *pos, void *stream);
+
+/* The cache: a pool of pages of `block` tokens (16, 32, 64 or 128). A page
+ * holds for each kv head block x head_dim codes and one scale, for K and for V;
+ * a code c stands for c * scale. k, v: [n_pages][n_head_kv][block][head_dim]
+ * bytes, 128-byte aligned; scales: [n_pages][n_head_kv]. head_dim 128 or 256.
+ * Token slot = page * block + place in the page. The pool needs no
+ * initialisation. */
+typedef enum {
+    CPQ_KV_INT8 = 0, /* -127 .. 127 */
+    CPQ_KV_E4M3 = 1, /* 8-bit floats, largest 448 */
+} cpq_kv_format;
+
+typedef struct cpq_kv_cache {
+    int32_t format, head_dim, n_head_kv, block;
+    int64_t n_pages;
+    void *k, *v;
+    float *k_scale, *v_scale;
+} cpq_kv_cache;
+
+/* Block tables and slot maps from the requests' lengths, on the device.
+ * Request r holds ctx_len[r] tokens in the pages table[r][0 ..] and gets
+ * new_len[r] more: pages for the blocks it does not hold yet are taken, in
+ * request order, from free_pages[*taken ..] and written to its table row;
+ * *taken_out = *taken + the pages taken. Outputs:
+ *   seq_start[n_seqs + 1]  first row of each request (sums of new_len), at most n_rows
+ *   kv_len[n_seqs]         ctx_len + new_len
+ *   pos[n_rows], slot[n_rows]  position and slot of each new token's row
+ * Rows behind the last request get pos 0 and slot -1. A request that cannot be
+ * served (too few free pages left, more than max_blocks blocks, rows past
+ * n_rows, a negative length) keeps its rows' place but gets kv_len 0, slots -1
+ * and no page; requests that need no page are served even then. Outputs must
+ * not overlap inputs, except table (in and out) and taken_out, which may be
+ * taken itself. */
+typedef struct cpq_kv_slot_args {
+    const int32_t *ctx_len, *new_len; /* [n_seqs] */
+    int64_t n_seqs;
+    int32_t *table;                   /* [n_seqs][table_stride] */
+    int64_t table_stride;
+    int32_t max_blocks, block;
+    const int32_t *free_pages;        /* [n_free] */
+    int64_t n_free;
+    const int32_t *taken;             /* [1] */
+    int32_t *taken_out;               /* [1] */
+    int32_t *seq_start, *kv_len, *pos;
+    int64_t *slot;
+    int64_t n_rows;
+} cpq_kv_slot_args;
+
+cpq_status cpq_kv_slots(const cpq_kv_slot_args *args, void *stream);
+
+/* Writes rows k, v (ne = [head_dim, n_head_kv, rows, 1]) to their slots. Rows
+ * whose slot is outside the pool (-1) are skipped. A run of rows with
+ * consecutive slots of one page is written together: the scale of a page and
+ * head becomes s = max|x| / 127 (int8) or / 448 (e4m3) over the run, rounded
+ * to fp32, or the old scale if that is larger and the run does not begin at
+ * the page's first place; codes are x / s rounded to nearest, ties to even.
+ * When s grows, the places before the run are coded again (c * s_old / s to
+ * nearest); the places after it are left as they are. NaN is stored as 0,
+ * infinities as the largest code, and neither counts for the scale; a scale
+ * under 2^-100 becomes 0. All rows of a call that go to one page must form one
+ * run: two runs in a page in one call leave it undefined. */
+cpq_status cpq_kv_append(const cpq_kv_cache *cache, const cpq_tensor *k, const cpq_tensor *v, const int64_t *slot,
+                         void *stream);
+
+/* The values (code * scale) of any slots, as rows of k and v (the shapes of
+ * cpq_kv_append); rows whose slot is outside the pool become zeros. */
+cpq_status cpq_kv_gather(const cpq_kv_cache *cache, const int64_t *slot, cpq_tensor *k, cpq_tensor *v, void *stream);
+
+/* The sequences of an attention call: rows seq_start[s] .. seq_start[s + 1] - 1
+ * of q are the last tokens of kv_len[s] cached ones, whose pages are
+ * table[s][0 ..] (device memory; at most 1024 sequences). */
+typedef struct cpq_attn_seqs {
+    const int32_t *seq_start; /* [n_seqs + 1], ascending */
+    const int32_t *kv_len;    /* [n_seqs] */
+    const int32_t *table;     /* [n_seqs][table_stride] */
+    int64_t table_stride;
+    int64_t n_seqs;
+    int32_t max_blocks;       /* blocks a table row has; keys beyond them are not seen */
+} cpq_attn_seqs;
+
+/* out = softmax(scale * q K^T) V over the cached keys (their values code *
+ * scale), q and out ne = [head_dim, n_head, tokens, 1] with n_head a multiple
+ * of n_head_kv (query head h reads kv head h / (n_head / n_head_kv)). causal:
+ * row i of a sequence's q_len rows sees the keys j < kv_len - q_len + i + 1;
+ * otherwise all kv_len (cross attention: any lengths). A row that sees no key
+ * gives 0; a table entry outside the pool makes its block's keys unseen. Rows
+ * of q outside every sequence leave their rows of out as they are. lse
+ * ([tokens][n_head] F32, or NULL) receives log sum exp of the scaled scores
+ * (-inf for a row that sees none). out must not overlap q. Sums are fp32; with
+ * F32 q the products carry 22 bits, with F16 and BF16 probabilities enter the
+ * second product in fp16. workspace: at least cpq_paged_attn_workspace_size
+ * bytes, 256-byte aligned, any contents, in use until the call has run: calls
+ * (and captured graphs) that may overlap on the GPU need workspaces of their
+ * own. */
+size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *cache, const cpq_tensor *q);
+cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *cache, const cpq_attn_seqs *seqs, float scale,
+                          int32_t causal, cpq_tensor *out, float *lse, void *workspace, size_t workspace_bytes,
+                          void *stream);
 
 /* ---- GGUF files: tensor directory and tensor-parallel shards ---------------
  *
