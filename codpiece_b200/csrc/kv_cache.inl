@@ -4,6 +4,19 @@ namespace cpq {
 
 static bool kv_block_ok(int32_t b) { return b == 16 || b == 32 || b == 64 || b == 128; }
 
+// Lets a kernel use `bytes` of dynamic shared memory, once per device.
+template <auto KERNEL>
+static cudaError_t raise_shared_limit(int bytes) {
+    static std::atomic<uint64_t> done{0};  // bit per device
+    const uint64_t bit = uint64_t(1) << (std::max(current_device(), 0) & 63);
+    if (done.load() & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
+}
+
+static int log_block(int32_t b) { return b == 16 ? 4 : b == 32 ? 5 : b == 64 ? 6 : 7; }
+
 // The cache's own fields; what: the caller's name in messages.
 static cpq_status check_cache(const cpq_kv_cache *c, const char *what) {
     if (!c) return fail(CPQ_ERR_INVALID_ARG, "%s: null cache", what);
@@ -35,16 +48,34 @@ static cpq_status check_kv_rows(const cpq_kv_cache *c, const cpq_tensor *k, cons
 
 static bool wide_rows(const cpq_tensor *t, size_t a) { return aligned(t->data, a) && t->nb[1] % a == 0 && t->nb[2] % a == 0; }
 
-template <typename T, int VEC>
-static cudaError_t launch_append(const AppendArgs &a, int fmt, dim3 grid, cudaStream_t st) {
-    return fmt == CPQ_KV_INT8 ? launch(kv_append_kernel<T, VEC, CPQ_KV_INT8>, grid, dim3(kAppendThreads), 0, st, a)
-                              : launch(kv_append_kernel<T, VEC, CPQ_KV_E4M3>, grid, dim3(kAppendThreads), 0, st, a);
+template <typename T, bool WIDE, int FMT>
+static cudaError_t launch_append_k(const AppendArgs &a, dim3 grid, cudaStream_t st) {
+    constexpr int kMax = 128 * 256 * int(sizeof(T));  // a run of the largest page
+    const int bytes = (a.d << a.log_block) * int(sizeof(T));
+    if (bytes > 48 * 1024) {
+        const cudaError_t e = raise_shared_limit<kv_append_kernel<T, WIDE, FMT>>(kMax);
+        if (e != cudaSuccess) return e;
+    }
+    const int items = bytes / 16;  // a thread has some items, a CTA not more threads than it needs
+    const dim3 block(unsigned(std::min(kAppendThreads, std::max(64, items / 8))));
+    return launch(kv_append_kernel<T, WIDE, FMT>, grid, block, size_t(bytes), st, a);
 }
 
-template <typename T, bool WIDE>
-static cudaError_t launch_gather(const GatherArgs &a, int fmt, dim3 grid, cudaStream_t st) {
-    return fmt == CPQ_KV_INT8 ? launch(kv_gather_kernel<T, WIDE, CPQ_KV_INT8>, grid, dim3(kGatherThreads), 0, st, a)
-                              : launch(kv_gather_kernel<T, WIDE, CPQ_KV_E4M3>, grid, dim3(kGatherThreads), 0, st, a);
+template <typename T>
+static cudaError_t launch_append(const AppendArgs &a, bool wide, int fmt, dim3 grid, cudaStream_t st) {
+    if (fmt == CPQ_KV_INT8)
+        return wide ? launch_append_k<T, true, CPQ_KV_INT8>(a, grid, st) : launch_append_k<T, false, CPQ_KV_INT8>(a, grid, st);
+    return wide ? launch_append_k<T, true, CPQ_KV_E4M3>(a, grid, st) : launch_append_k<T, false, CPQ_KV_E4M3>(a, grid, st);
+}
+
+template <typename T>
+static cudaError_t launch_gather(const GatherArgs &a, bool wide, int fmt, dim3 grid, cudaStream_t st) {
+    const dim3 block(kGatherThreads);
+    if (fmt == CPQ_KV_INT8)
+        return wide ? launch(kv_gather_kernel<T, true, CPQ_KV_INT8>, grid, block, 0, st, a)
+                    : launch(kv_gather_kernel<T, false, CPQ_KV_INT8>, grid, block, 0, st, a);
+    return wide ? launch(kv_gather_kernel<T, true, CPQ_KV_E4M3>, grid, block, 0, st, a)
+                : launch(kv_gather_kernel<T, false, CPQ_KV_E4M3>, grid, block, 0, st, a);
 }
 
 }  // namespace cpq
@@ -67,8 +98,8 @@ extern "C" cpq_status cpq_kv_slots(const cpq_kv_slot_args *s, void *stream) {
     if (s->n_free > 0 && !s->free_pages) return fail(CPQ_ERR_INVALID_ARG, "kv_slots: null free_pages");
     SlotArgs a{s->ctx_len, s->new_len, s->n_seqs, s->table, s->table_stride, s->max_blocks, s->block,
                s->free_pages, s->n_free, s->taken, s->taken_out, s->seq_start, s->kv_len, s->pos, s->slot, s->n_rows};
-    // one CTA writes some thousand rows in about the time of the scan; more need company
-    const int64_t per_cta = 4096;
+    // a row per thread; the scan, which every CTA repeats, takes longer than that
+    const int64_t per_cta = 1024;
     int64_t ctas = s->taken_out == s->taken ? 1 : (s->n_rows + per_cta - 1) / per_cta;
     ctas = std::min<int64_t>(std::max<int64_t>(ctas, 1), sm_count(std::max(current_device(), 0)));
     const cudaError_t e = launch(kv_slots_kernel, dim3(unsigned(ctas)), dim3(kSlotThreads), 0, static_cast<cudaStream_t>(stream), a);
@@ -101,19 +132,18 @@ extern "C" cpq_status cpq_kv_append(const cpq_kv_cache *c, const cpq_tensor *k, 
     a.n_slots = c->n_pages * c->block;
     a.n_head = c->n_head_kv;
     a.d = c->head_dim;
-    a.block = c->block;
-    a.group = 1;
+    a.log_block = log_block(c->block);
+    // A group's runs are written one after another, so few rows get a CTA each; many rows are mostly
+    // insides of runs, whose CTAs would only look and leave.
+    const int64_t work = t * c->n_head_kv * 2, sms = sm_count(std::max(current_device(), 0));
+    a.group = int(std::min<int64_t>(kAppendMaxGroup, std::max<int64_t>(1, work / (16 * sms))));
     const dim3 grid(unsigned((t + a.group - 1) / a.group), unsigned(c->n_head_kv), 2);
     const bool wide = wide_rows(k, 16) && wide_rows(v, 16);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (k->type == CPQ_TYPE_F32)
-        e = wide ? launch_append<float, 4>(a, c->format, grid, s) : launch_append<float, 1>(a, c->format, grid, s);
-    else if (k->type == CPQ_TYPE_F16)
-        e = wide ? launch_append<__half, 8>(a, c->format, grid, s) : launch_append<__half, 1>(a, c->format, grid, s);
-    else
-        e = wide ? launch_append<__nv_bfloat16, 8>(a, c->format, grid, s)
-                 : launch_append<__nv_bfloat16, 1>(a, c->format, grid, s);
+    if (k->type == CPQ_TYPE_F32) e = launch_append<float>(a, wide, c->format, grid, s);
+    else if (k->type == CPQ_TYPE_F16) e = launch_append<__half>(a, wide, c->format, grid, s);
+    else e = launch_append<__nv_bfloat16>(a, wide, c->format, grid, s);
     return e == cudaSuccess ? CPQ_SUCCESS : cuda_fail(e, "kv_append launch");
 }
 
@@ -142,14 +172,14 @@ extern "C" cpq_status cpq_kv_gather(const cpq_kv_cache *c, const int64_t *slot, 
     a.n_slots = c->n_pages * c->block;
     a.n_head = c->n_head_kv;
     a.d = c->head_dim;
-    a.block = c->block;
-    const int64_t items = t * c->n_head_kv * (c->head_dim / 16);
-    const dim3 grid(unsigned(std::min<int64_t>((items + kGatherThreads - 1) / kGatherThreads, 1 << 20)), 2);
+    a.log_block = log_block(c->block);
+    a.by_row = FastDiv(uint32_t(c->n_head_kv) * uint32_t(c->head_dim) / uint32_t(16 / b));
+    const dim3 grid(unsigned((t + kGatherRows - 1) / kGatherRows), 2);
     const bool wide = wide_rows(k, 16) && wide_rows(v, 16);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (k->type == CPQ_TYPE_F32) e = wide ? launch_gather<float, true>(a, c->format, grid, s) : launch_gather<float, false>(a, c->format, grid, s);
-    else if (k->type == CPQ_TYPE_F16) e = wide ? launch_gather<__half, true>(a, c->format, grid, s) : launch_gather<__half, false>(a, c->format, grid, s);
-    else e = wide ? launch_gather<__nv_bfloat16, true>(a, c->format, grid, s) : launch_gather<__nv_bfloat16, false>(a, c->format, grid, s);
+    if (k->type == CPQ_TYPE_F32) e = launch_gather<float>(a, wide, c->format, grid, s);
+    else if (k->type == CPQ_TYPE_F16) e = launch_gather<__half>(a, wide, c->format, grid, s);
+    else e = launch_gather<__nv_bfloat16>(a, wide, c->format, grid, s);
     return e == cudaSuccess ? CPQ_SUCCESS : cuda_fail(e, "kv_gather launch");
 }

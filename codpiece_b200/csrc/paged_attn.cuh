@@ -328,23 +328,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes (bytes 0, 1) and (bytes 2, 3) of w as fp16 pairs, exact. int8: 0x6400 |
-// (code + 128) is 1152 + code.
-template <int FMT>
-__device__ __forceinline__ void codes_h2(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (FMT == CPQ_KV_INT8) {
-        w ^= 0x80808080u;
-        const __half2 k1152 = __float2half2_rn(1152.0f);
-        lo = h2u(__hsub2(u32_h2(__byte_perm(w, 0x64646464u, 0x4140)), k1152));
-        hi = h2u(__hsub2(u32_h2(__byte_perm(w, 0x64646464u, 0x4342)), k1152));
-    } else {
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
-            "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-            : "=r"(lo), "=r"(hi)
-            : "r"(w));
-    }
-}
-
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) { return h2u(__floats2half2_rn(a, b)); }
 
 __device__ __forceinline__ void dec_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kAttnWarps) : "memory"); }

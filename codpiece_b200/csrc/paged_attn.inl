@@ -35,15 +35,9 @@ static void attn_carve(AttnArgs &a, void *ws, int ctas, int rows, int d) {
 template <int D, int FMT, bool SPLIT>
 static cudaError_t launch_attn_decode(const AttnArgs &a, int ctas, cudaStream_t st) {
     using C = DecCfg<D, SPLIT>;
-    static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised
-    const int dev = std::max(current_device(), 0);
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (!(set.load() & bit)) {
-        const cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, FMT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
-        if (e != cudaSuccess) return e;
-        set.fetch_or(bit);
-    }
-    cudaError_t e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kAttnThreads), C::kSmem, st, a);
+    cudaError_t e = raise_shared_limit<attn_decode_kernel<D, FMT, SPLIT>>(C::kSmem);
+    if (e != cudaSuccess) return e;
+    e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kAttnThreads), C::kSmem, st, a);
     if (e != cudaSuccess) return e;
     return launch(attn_combine_kernel<D, C::kRows>, dim3(unsigned(ctas), unsigned(C::kRows)), dim3(kCombineThreads), 0, st, a);
 }

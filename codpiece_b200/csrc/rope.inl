@@ -36,14 +36,14 @@ static bool head_rows(const cpq_tensor *t) {
 }
 
 template <typename T, int VEC>
-static cudaError_t launch_rope_v(const RopeArgs &a, bool half, dim3 grid, size_t smem, cudaStream_t st) {
-    return half ? launch(rope_kernel<T, VEC, true>, grid, dim3(kRopeThreads), smem, st, a)
-                : launch(rope_kernel<T, VEC < 2 ? 2 : VEC, false>, grid, dim3(kRopeThreads), smem, st, a);
+static cudaError_t launch_rope_v(const RopeArgs &a, bool half, dim3 grid, cudaStream_t st) {
+    return half ? launch(rope_kernel<T, VEC, true>, grid, dim3(kRopeThreads), 0, st, a)
+                : launch(rope_kernel<T, VEC < 2 ? 2 : VEC, false>, grid, dim3(kRopeThreads), 0, st, a);
 }
 
 template <typename T>
-static cudaError_t launch_rope(const RopeArgs &a, bool half, bool wide, dim3 grid, size_t smem, cudaStream_t st) {
-    return wide ? launch_rope_v<T, 16 / sizeof(T)>(a, half, grid, smem, st) : launch_rope_v<T, 1>(a, half, grid, smem, st);
+static cudaError_t launch_rope(const RopeArgs &a, bool half, bool wide, dim3 grid, cudaStream_t st) {
+    return wide ? launch_rope_v<T, 16 / sizeof(T)>(a, half, grid, st) : launch_rope_v<T, 1>(a, half, grid, st);
 }
 
 }  // namespace cpq
@@ -134,23 +134,31 @@ extern "C" cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *con
         return fail(CPQ_ERR_UNSUPPORTED, "rope: interleaved pairs need an even head size (%lld)", (long long)d);
     }
     a.pos = pos;
-    a.t = t;
     a.d = int(d);
     a.n_dims = rope->n_dims;
     a.n_tensors = n;
-    a.copy_tail = copy ? 1 : 0;
     a.m = rope->m;
     memcpy(a.turns, rope->turns, sizeof a.turns);
-    const int heads = a.head0[n];
-    a.tok_per_cta = 1;
-    a.heads_per_cta = heads;
-    const dim3 grid(unsigned(t), 1);
+    const int width = wide ? vec : half ? 1 : 2;  // elements of an item
+    a.pair_items = half ? rope->n_dims / 2 / width : (rope->n_dims + width - 1) / width;
+    a.items = a.pair_items + (copy ? int(d - (half ? rope->n_dims : a.pair_items * width)) / width : 0);
     if (t > 2147483647) return fail(CPQ_ERR_UNSUPPORTED, "rope: %lld tokens", (long long)t);
-    const size_t smem = size_t(a.tok_per_cta) * size_t(rope->n_dims / 2) * sizeof(float2);
+    // a CTA takes one token's heads, or several tokens' once that still gives every SM its CTAs; few tokens
+    // share their heads out over as many CTAs as fill the GPU, down to about one item per thread
+    const int heads = a.head0[n], least = std::min(heads, (kRopeThreads + a.items - 1) / a.items);
+    const int64_t sms = sm_count(std::max(current_device(), 0));
+    const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(heads / least, 2 * sms / t));
+    a.heads_per_cta = int((heads + groups - 1) / groups);
+    a.tok_per_cta = t >= 20 * sms ? 4 : t >= 10 * sms ? 2 : 1;
+    a.t = t;
+    a.by_items = FastDiv(uint32_t(a.items));
+    a.step = std::max(1, kRopeThreads / a.items);
+    a.by_pairs = FastDiv(uint32_t(rope->n_dims / 2));
+    const dim3 grid(unsigned((t + a.tok_per_cta - 1) / a.tok_per_cta), unsigned((heads + a.heads_per_cta - 1) / a.heads_per_cta));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (x[0]->type == CPQ_TYPE_F32) e = launch_rope<float>(a, half, wide, grid, smem, st);
-    else if (x[0]->type == CPQ_TYPE_F16) e = launch_rope<__half>(a, half, wide, grid, smem, st);
-    else e = launch_rope<__nv_bfloat16>(a, half, wide, grid, smem, st);
+    if (x[0]->type == CPQ_TYPE_F32) e = launch_rope<float>(a, half, wide, grid, st);
+    else if (x[0]->type == CPQ_TYPE_F16) e = launch_rope<__half>(a, half, wide, grid, st);
+    else e = launch_rope<__nv_bfloat16>(a, half, wide, grid, st);
     return e == cudaSuccess ? CPQ_SUCCESS : cuda_fail(e, "rope launch");
 }
