@@ -143,7 +143,7 @@ def lib() -> C.CDLL:
         "cpq_kv_slots": (st, [P(CpqKvSlotArgs), vp]),
         "cpq_kv_append": (st, [P(CpqKvCache), P(CpqTensor), P(CpqTensor), vp, vp]),
         "cpq_kv_gather": (st, [P(CpqKvCache), vp, P(CpqTensor), P(CpqTensor), vp]),
-        "cpq_paged_attn_workspace_size": (sz, [P(CpqKvCache), P(CpqTensor)]),
+        "cpq_paged_attn_workspace_size": (sz, [P(CpqKvCache), P(CpqTensor), i64]),
         "cpq_paged_attn": (st, [P(CpqTensor), P(CpqKvCache), P(CpqAttnSeqs), C.c_float, i32, P(CpqTensor), vp, vp, sz,
                                 vp]),
         "cpq_decode_plan_create": (st, [P(CpqDecodePhase), C.c_int, C.c_int, P(vp)]),

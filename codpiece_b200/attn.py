@@ -288,7 +288,7 @@ def paged_attn(q: torch.Tensor, cache: KvCache, table: torch.Tensor, seq_start: 
             out = torch.empty(q.shape, dtype=q.dtype, device=dev)
         if lse is None and return_lse:
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-        need = lib().cpq_paged_attn_workspace_size(C.byref(cd), C.byref(qd))
+        need = lib().cpq_paged_attn_workspace_size(C.byref(cd), C.byref(qd), n)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     _same_device(dev, out=out, lse=lse, workspace=workspace)

@@ -16,7 +16,8 @@
 //   gdn.cuh          gated delta-net recurrence (the GDN layers' per-token state update)
 //   rope.cuh         rotary positions
 //   kv_cache.cuh     paged 8-bit key/value cache: slot maps, append, gather
-//   paged_attn.cuh   attention over the paged cache
+//   paged_attn.cuh   attention over the paged cache: the split, and few query rows (decode)
+//   paged_attn_tc.cuh the same for many query rows (verify, prefill) on tcgen05 tensor cores
 //   elementwise.cuh  rms norm, SwiGLU, residual add, argmax
 //   synth.cuh        seeded synthetic weights
 //   split.inl        tensor-parallel partition rules (host)
@@ -56,6 +57,7 @@
 #include "rope.cuh"
 #include "kv_cache.cuh"
 #include "paged_attn.cuh"
+#include "paged_attn_tc.cuh"
 #include "quantize.cuh"
 #include "synth.cuh"
 #include "split.inl"

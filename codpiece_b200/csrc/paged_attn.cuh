@@ -49,6 +49,7 @@ struct alignas(64) AttnArgs {
     int64_t os_tok, os_head;
     float *lse;                  // [t][hkv * group], or null
     int type;                    // of q and out
+    int wide;                    // q and out: 16-byte aligned rows
     int t, group, n_seqs;
     const int32_t *seq_start, *kv_len, *table;
     int64_t table_stride;
@@ -94,8 +95,10 @@ struct AttnPlan {
 
 // Fills the plan (all threads of the CTA; two barriers inside). A unit with no
 // visible key counts one tile, so that some CTA writes its rows.
+// Also marks the CTA's workspace slots unused, before any is written.
 template <int ROWS, int TILE>
 __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
+    if (threadIdx.x < 2) a.part_hdr[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
     auto tiles = [&](const AttnSeq &s, int r) {
         return max(1, (attn_kv_end(s, r, ROWS, a.group, a.causal) + TILE - 1) / TILE);
@@ -218,12 +221,6 @@ struct AttnWalk {
 
 // The workspace slot of a cut unit: 0 when it began in an earlier CTA, 1 when it begins here.
 __device__ __forceinline__ int attn_slot(const AttnUnit &u) { return 2 * int(blockIdx.x) + (u.t0 == 0 ? 1 : 0); }
-
-// Marks both of this CTA's slots unused, before any is written.
-__device__ __forceinline__ void attn_clear_slots(const AttnArgs &a) {
-    a.part_hdr[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-    a.part_hdr[2 * blockIdx.x + 1] = make_int4(0, 0, 0, 0);
-}
 
 // The page of a sequence's block b, or -1 when it is no page of the pool (its
 // keys then count as absent).
@@ -358,7 +355,6 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
     pdl_wait();
     pdl_launch_dependents();
     attn_make_plan<kRows, kAttnTile>(a, plan);
-    if (threadIdx.x == 0) attn_clear_slots(a);
     AttnWalk<kRows, kAttnTile> walk(a, plan);
     AttnUnit u;
     const int lb = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
@@ -721,29 +717,36 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
 
 // ---- joining a cut unit ------------------------------------------------------------
 //
-// grid (CTAs of the attention grid, rows): block (c, rr) joins row rr of the
-// unit that begins in CTA c and goes on in c + 1, ...: sum over the parts of
-// part * 2^(reference - largest reference). D / 4 threads across, the parts
-// dealt out over the rest of the block and added in a fixed order.
+// grid (CTAs of the attention grid, rows / ROWS_HERE): block (c, y) joins rows
+// of the unit that begins in CTA c and goes on in c + 1, ...: sum over the parts
+// of part * 2^(reference - largest reference). D / 4 threads across a row; with
+// few rows the parts are dealt out over the rest of the block and added in a
+// fixed order.
 
 constexpr int kCombineThreads = 256;
 
+template <int D, int ROWS> struct CombineCfg {
+    static constexpr int kAcross = D / 4, kSets = kCombineThreads / kAcross;
+    static constexpr int kRowsHere = ROWS > 16 ? kSets : 1;  // rows of a block
+    static constexpr int kDeal = kSets / kRowsHere;          // sets that share a row's parts
+};
+
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kCombineThreads) attn_combine_kernel(const __grid_constant__ AttnArgs a) {
-    constexpr int kAcross = D / 4, kDeal = kCombineThreads / kAcross;
-    __shared__ float4 s_o[kDeal][kAcross];
-    __shared__ float s_l[kDeal];
-    const int c = blockIdx.x, rr = blockIdx.y;
-    const int x = threadIdx.x % kAcross, z = threadIdx.x / kAcross;
+    using C = CombineCfg<D, ROWS>;
+    __shared__ float4 s_o[C::kSets][C::kAcross];
+    __shared__ float s_l[C::kSets];
+    __shared__ int s_n;
+    const int c = blockIdx.x;
+    const int x = threadIdx.x % C::kAcross, set = threadIdx.x / C::kAcross;
+    const int rr = blockIdx.y * C::kRowsHere + set / C::kDeal, z = set % C::kDeal;
     pdl_wait();
     pdl_launch_dependents();
     const int4 hdr = a.part_hdr[2 * c + 1];
     if (hdr.w == 0) return;
     const AttnSeq seq = attn_seq(a, hdr.x);
-    const int row = hdr.y * ROWS + rr;
-    if (row >= seq.q * a.group) return;
+    if (hdr.y * ROWS + int(blockIdx.y) * C::kRowsHere >= seq.q * a.group) return;
     // parts: slot 2c + 1, then 2(c + 1), 2(c + 2), ... up to the one that ends the unit
-    __shared__ int s_n;
     if (threadIdx.x == 0) s_n = int(gridDim.x) - c;
     __syncthreads();
     for (int i = threadIdx.x; i < int(gridDim.x) - c; i += kCombineThreads) {
@@ -753,38 +756,37 @@ __global__ void __launch_bounds__(kCombineThreads) attn_combine_kernel(const __g
     __syncthreads();
     const int n = s_n;
     auto slot = [&](int i) { return int64_t(i == 0 ? 2 * c + 1 : 2 * (c + i)); };
-    __shared__ float s_m[kCombineThreads / 32];
     float m = __int_as_float(0xff800000);
-    for (int i = threadIdx.x; i < n; i += kCombineThreads) m = fmaxf(m, a.part_ml[slot(i) * ROWS + rr].x);
+    for (int i = threadIdx.x & 31; i < n; i += 32) m = fmaxf(m, a.part_ml[slot(i) * ROWS + rr].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; w++) m = fmaxf(m, s_m[w]);
     const float b = m == __int_as_float(0xff800000) ? 0.0f : m;
     float4 acc = make_float4(0, 0, 0, 0);
     float l = 0.0f;
 #pragma unroll 4
-    for (int i = z; i < n; i += kDeal) {
+    for (int i = z; i < n; i += C::kDeal) {
         const float2 ml = a.part_ml[slot(i) * ROWS + rr];
         const float4 v = *reinterpret_cast<const float4 *>(a.part_o + (slot(i) * ROWS + rr) * D + 4 * x);
         const float f = ex2(ml.x - b);
         acc.x += v.x * f, acc.y += v.y * f, acc.z += v.z * f, acc.w += v.w * f;
         l += ml.y * f;
     }
-    s_o[z][x] = acc;
-    if (x == 0) s_l[z] = l;
-    __syncthreads();
-    if (z) return;
-    l = 0.0f;
-    acc = make_float4(0, 0, 0, 0);
+    if constexpr (C::kDeal > 1) {
+        s_o[set][x] = acc;
+        if (x == 0) s_l[set] = l;
+        __syncthreads();
+        if (z) return;
+        l = 0.0f;
+        acc = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kDeal; i++) {
-        const float4 v = s_o[i][x];
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-        l += s_l[i];
+        for (int i = 0; i < C::kDeal; i++) {
+            const float4 v = s_o[set + i][x];
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            l += s_l[set + i];
+        }
     }
+    const int row = hdr.y * ROWS + rr;
+    if (row >= seq.q * a.group) return;
     const float f = attn_inverse(l);
     const int tok = seq.row0 + row / a.group, head = hdr.z * a.group + row % a.group;
     const int64_t to = tok * a.os_tok + head * a.os_head + 4 * x;

@@ -1,4 +1,4 @@
-// paged_attn.inl — cpq_paged_attn: host side of paged_attn.cuh.
+// paged_attn.inl — cpq_paged_attn: host side of paged_attn.cuh and paged_attn_tc.cuh.
 
 namespace cpq {
 
@@ -32,6 +32,12 @@ static void attn_carve(AttnArgs &a, void *ws, int ctas, int rows, int d) {
     a.part_hdr = reinterpret_cast<int4 *>(p);
 }
 
+template <int D, int ROWS>
+static cudaError_t launch_attn_combine(const AttnArgs &a, int ctas, cudaStream_t st) {
+    constexpr int y = ROWS / CombineCfg<D, ROWS>::kRowsHere;
+    return launch(attn_combine_kernel<D, ROWS>, dim3(unsigned(ctas), unsigned(y)), dim3(kCombineThreads), 0, st, a);
+}
+
 template <int D, int FMT, bool SPLIT>
 static cudaError_t launch_attn_decode(const AttnArgs &a, int ctas, cudaStream_t st) {
     using C = DecCfg<D, SPLIT>;
@@ -39,21 +45,40 @@ static cudaError_t launch_attn_decode(const AttnArgs &a, int ctas, cudaStream_t 
     if (e != cudaSuccess) return e;
     e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kAttnThreads), C::kSmem, st, a);
     if (e != cudaSuccess) return e;
-    return launch(attn_combine_kernel<D, C::kRows>, dim3(unsigned(ctas), unsigned(C::kRows)), dim3(kCombineThreads), 0, st, a);
+    return launch_attn_combine<D, C::kRows>(a, ctas, st);
+}
+
+template <int D, int FMT, bool SPLIT>
+static cudaError_t launch_attn_tc(const AttnArgs &a, int ctas, cudaStream_t st) {
+    using C = TaCfg<D, SPLIT>;
+    cudaError_t e = raise_shared_limit<attn_tc_kernel<D, FMT, SPLIT>>(C::kSmem);
+    if (e != cudaSuccess) return e;
+    e = launch(attn_tc_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kTaThreads), C::kSmem, st, a);
+    if (e != cudaSuccess) return e;
+    return launch_attn_combine<D, kTaRows>(a, ctas, st);
 }
 
 template <int D, bool SPLIT>
-static cudaError_t launch_attn_fmt(const AttnArgs &a, int fmt, int ctas, cudaStream_t st) {
-    return fmt == CPQ_KV_INT8 ? launch_attn_decode<D, CPQ_KV_INT8, SPLIT>(a, ctas, st)
-                              : launch_attn_decode<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st);
+static cudaError_t launch_attn(const AttnArgs &a, bool tc, int fmt, int ctas, cudaStream_t st) {
+    if (fmt == CPQ_KV_INT8)
+        return tc ? launch_attn_tc<D, CPQ_KV_INT8, SPLIT>(a, ctas, st) : launch_attn_decode<D, CPQ_KV_INT8, SPLIT>(a, ctas, st);
+    return tc ? launch_attn_tc<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st) : launch_attn_decode<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st);
+}
+
+// The rows of a row tile: the decode kernel's while the sequences' query rows
+// (tokens x heads of a group) fill no more than one of its tiles on average,
+// else the tensor-core kernel's.
+static int attn_rows(const cpq_tensor *q, const cpq_kv_cache *c, int64_t n_seqs) {
+    const int few = q->type == CPQ_TYPE_F32 ? 8 : 16;
+    return q->ne[2] * (q->ne[1] / c->n_head_kv) <= few * n_seqs ? few : kTaRows;
 }
 
 }  // namespace cpq
 
-extern "C" size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *c, const cpq_tensor *q) {
+extern "C" size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *c, const cpq_tensor *q, int64_t n_seqs) {
     using namespace cpq;
-    if (!c || !q) return 0;
-    return attn_ws_bytes(sm_count(std::max(current_device(), 0)), 16, c->head_dim);
+    if (!c || !q || c->n_head_kv < 1) return 0;
+    return attn_ws_bytes(sm_count(std::max(current_device(), 0)), attn_rows(q, c, n_seqs), c->head_dim);
 }
 
 extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c, const cpq_attn_seqs *s, float scale,
@@ -81,9 +106,11 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     if (rows > 2147483647 || c->n_pages * c->n_head_kv * c->block > 2147483647 || int64_t(s->max_blocks) * c->block > 2147483647)
         return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: more than 2^31 - 1 rows, cache rows or keys");
     const bool split = q->type == CPQ_TYPE_F32;
-    const int unit_rows = split ? 8 : 16;
+    const int unit_rows = attn_rows(q, c, s->n_seqs);
+    const bool tc = unit_rows == kTaRows;
     // the units' tiles are counted in 32 bits
-    const int64_t tiles = std::max<int64_t>(1, (int64_t(s->max_blocks) * c->block + kAttnTile - 1) / kAttnTile);
+    const int tile = tc ? kTaTile : kAttnTile;
+    const int64_t tiles = std::max<int64_t>(1, (int64_t(s->max_blocks) * c->block + tile - 1) / tile);
     if ((rows / unit_rows + s->n_seqs * c->n_head_kv) > 2147483647 / tiles)
         return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: %lld rows over up to %lld keys are too many for one call", (long long)rows,
                     (long long)s->max_blocks * c->block);
@@ -122,11 +149,12 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     a.max_blocks = s->max_blocks;
     a.causal = causal ? 1 : 0;
     a.scale_log2 = float(double(scale) * 1.4426950408889634);
-    a.min_tiles = kAttnWarps;
+    a.wide = wide_rows(q, 16) && wide_rows(out, 16) ? 1 : 0;
+    a.min_tiles = tc ? 4 : kAttnWarps;
     attn_carve(a, workspace, ctas, unit_rows, c->head_dim);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
     cudaError_t e;
-    if (c->head_dim == 256) e = split ? launch_attn_fmt<256, true>(a, c->format, ctas, cs) : launch_attn_fmt<256, false>(a, c->format, ctas, cs);
-    else e = split ? launch_attn_fmt<128, true>(a, c->format, ctas, cs) : launch_attn_fmt<128, false>(a, c->format, ctas, cs);
+    if (c->head_dim == 256) e = split ? launch_attn<256, true>(a, tc, c->format, ctas, cs) : launch_attn<256, false>(a, tc, c->format, ctas, cs);
+    else e = split ? launch_attn<128, true>(a, tc, c->format, ctas, cs) : launch_attn<128, false>(a, tc, c->format, ctas, cs);
     return e == cudaSuccess ? CPQ_SUCCESS : cuda_fail(e, "paged_attn launch");
 }

@@ -533,7 +533,7 @@ typedef struct cpq_attn_seqs {
  * bytes, 256-byte aligned, any contents, in use until the call has run: calls
  * (and captured graphs) that may overlap on the GPU need workspaces of their
  * own. */
-size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *cache, const cpq_tensor *q);
+size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *cache, const cpq_tensor *q, int64_t n_seqs);
 cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *cache, const cpq_attn_seqs *seqs, float scale,
                           int32_t causal, cpq_tensor *out, float *lse, void *workspace, size_t workspace_bytes,
                           void *stream);

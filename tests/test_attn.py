@@ -172,7 +172,7 @@ def test_paged_attn_refuses(L):
     assert call(n_ws=1000) == WORKSPACE and call(ws=0x80010) == WORKSPACE
     assert call(q=tensor(256, 24, 0), out=tensor(256, 24, 0)) == OK               # no tokens
     assert call(n_seqs=0) == OK
-    assert L.cpq_paged_attn_workspace_size(None, None) == 0
+    assert L.cpq_paged_attn_workspace_size(None, None, 1) == 0
 
 
 def test_python_surface_refuses_cpu_tensors():
