@@ -13,10 +13,11 @@
 // exactly; an fp32 value takes two (22 bits, the second the rounding error of
 // the first). Probabilities enter the second product the same way: one fp16
 // term for 16-bit outputs, two for fp32. The softmax reference of a row is
-// kept 8 (in log2) under the running maximum and moves when a score exceeds it
-// by more than 11, so probabilities lie in [0, 2^11] and small ones keep their
-// bits; a page's v_scale enters as its ratio to a reference scale, which moves
-// when a ratio exceeds 8. Sums are fp32.
+// set 2 (in log2) under a maximum and moves when a score exceeds it by more than
+// 12, so probabilities lie in [0, 2^12] and it moves once or twice in a row's
+// life (with 8 and 11 some row of a warp moved in every second or third tile,
+// and each time O is rescaled); a page's v_scale enters as its ratio to a
+// reference scale, which moves when a ratio exceeds 8. Sums are fp32.
 //
 // Work. The query rows of one kv head and sequence, (token, head of the group)
 // in that order, form row tiles of kRows rows; a unit is (sequence, row tile,
@@ -85,19 +86,17 @@ __device__ __forceinline__ int attn_kv_end(const AttnSeq &s, int r, int rows, in
 
 __device__ __forceinline__ int attn_row_tiles(const AttnSeq &s, int rows, int group) { return (s.q * group + rows - 1) / rows; }
 
-// A CTA's share of the tiles, and the units in it in order.
+// Where a CTA's share of the tiles begins.
 struct AttnPlan {
-    AttnSeq seq[kAttnMaxSeqs];
-    int through[kAttnMaxSeqs + 1];  // tiles before each sequence
-    int s, r, h, tile, left;        // where this CTA begins, and its tiles
-    int n_cta;                      // CTAs that have a share
+    int s, r, h, tile, left;  // unit and tile, and the share's tiles
 };
 
-// Fills the plan (all threads of the CTA; two barriers inside). A unit with no
-// visible key counts one tile, so that some CTA writes its rows.
-// Also marks the CTA's workspace slots unused, before any is written.
+// Fills the plan (all threads of the CTA; barriers inside). through: scratch of
+// kAttnMaxSeqs + 1 ints, free again afterwards. A unit with no visible key
+// counts one tile, so that some CTA writes its rows. Also marks the CTA's
+// workspace slots unused, before any is written.
 template <int ROWS, int TILE>
-__device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
+__device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, int *through) {
     if (threadIdx.x < 2) a.part_hdr[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
     auto tiles = [&](const AttnSeq &s, int r) {
@@ -105,41 +104,40 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
     };
     for (int s = tid; s < a.n_seqs; s += blockDim.x) {
         const AttnSeq q = attn_seq(a, s);
-        p.seq[s] = q;
         const int n = attn_row_tiles(q, ROWS, a.group);
         int w = -1;  // many row tiles: counted by a warp below
         if (n <= 4) {
             w = 0;
             for (int r = 0; r < n; r++) w += tiles(q, r);
         }
-        p.through[s + 1] = w < 0 ? -1 : w * a.hkv;
+        through[s + 1] = w < 0 ? -1 : w * a.hkv;
     }
     __syncthreads();
     for (int s = warp; s < a.n_seqs; s += n_warps) {
-        if (p.through[s + 1] >= 0) continue;
-        const AttnSeq q = p.seq[s];
+        if (through[s + 1] >= 0) continue;
+        const AttnSeq q = attn_seq(a, s);
         const int n = attn_row_tiles(q, ROWS, a.group);
         int w = 0;
         for (int r = lane; r < n; r += 32) w += tiles(q, r);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
         __syncwarp();
-        if (lane == 0) p.through[s + 1] = w * a.hkv;
+        if (lane == 0) through[s + 1] = w * a.hkv;
     }
     __syncthreads();
     if (warp == 0) {
         int sum = 0;
         for (int s0 = 0; s0 < a.n_seqs; s0 += 32) {
-            int w = s0 + lane < a.n_seqs ? p.through[s0 + lane + 1] : 0;
+            int w = s0 + lane < a.n_seqs ? through[s0 + lane + 1] : 0;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int u = __shfl_up_sync(0xffffffffu, w, o);
                 if (lane >= o) w += u;
             }
-            if (s0 + lane < a.n_seqs) p.through[s0 + lane + 1] = sum + w;
+            if (s0 + lane < a.n_seqs) through[s0 + lane + 1] = sum + w;
             sum += __shfl_sync(0xffffffffu, w, 31);
         }
-        if (lane == 0) p.through[0] = 0;
+        if (lane == 0) through[0] = 0;
         __syncwarp();
         const int n_cta = max(1, min(int(gridDim.x), sum / a.min_tiles));
         const int c = blockIdx.x;
@@ -147,15 +145,15 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
         const int x1 = c < n_cta ? int(int64_t(sum) * (c + 1) / n_cta) : sum;
         int s = 0, r = 0, h = 0, tile = 0;
         if (x1 > x0) {
-            int lo = 0, hi = a.n_seqs;  // the last sequence that begins at or before x0 and has tiles there
+            int lo = 0, hi = a.n_seqs;  // the last sequence that begins at or before x0 (and so has tiles there)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
-                if (p.through[mid] <= x0) lo = mid;
+                if (through[mid] <= x0) lo = mid;
                 else hi = mid;
             }
             s = lo;
-            int rem = x0 - p.through[s];
-            const AttnSeq q = p.seq[s];
+            int rem = x0 - through[s];
+            const AttnSeq q = attn_seq(a, s);
             const int n = attn_row_tiles(q, ROWS, a.group);
             for (int r0 = 0; r0 < n; r0 += 32) {  // row tiles in order, each with its hkv units
                 const int mine = r0 + lane < n ? tiles(q, r0 + lane) * a.hkv : 0;
@@ -178,7 +176,7 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p) {
                 rem -= __shfl_sync(0xffffffffu, w, 31);
             }
         }
-        if (lane == 0) p.s = s, p.r = r, p.h = h, p.tile = tile, p.left = x1 - x0, p.n_cta = n_cta;
+        if (lane == 0) p.s = s, p.r = r, p.h = h, p.tile = tile, p.left = x1 - x0;
     }
     __syncthreads();
 }
@@ -194,14 +192,16 @@ struct AttnUnit {
 template <int ROWS, int TILE>
 struct AttnWalk {
     const AttnArgs &a;
-    const AttnPlan &p;
     int s, r, h, tile, left;
-    __device__ AttnWalk(const AttnArgs &a_, const AttnPlan &p_) : a(a_), p(p_), s(p_.s), r(p_.r), h(p_.h), tile(p_.tile), left(p_.left) {}
+    AttnSeq seq;
+    __device__ AttnWalk(const AttnArgs &a_, const AttnPlan &p) : a(a_), s(p.s), r(p.r), h(p.h), tile(p.tile), left(p.left) {
+        if (left > 0) seq = attn_seq(a, s);
+    }
     __device__ bool next(AttnUnit &u) {
         if (left <= 0) return false;
         u.s = s, u.r = r, u.h = h;
-        u.seq = p.seq[s];
-        u.kv_end = attn_kv_end(u.seq, r, ROWS, a.group, a.causal);
+        u.seq = seq;
+        u.kv_end = attn_kv_end(seq, r, ROWS, a.group, a.causal);
         u.n = max(1, (u.kv_end + TILE - 1) / TILE);
         u.t0 = tile;
         u.t1 = min(u.n, tile + left);
@@ -209,10 +209,12 @@ struct AttnWalk {
         tile = 0;
         if (++h == a.hkv) {
             h = 0;
-            if (++r == attn_row_tiles(u.seq, ROWS, a.group)) {
+            if (++r == attn_row_tiles(seq, ROWS, a.group)) {
                 r = 0;
-                do s++;
-                while (s < a.n_seqs && p.seq[s].q == 0);
+                while (left > 0 && ++s < a.n_seqs) {
+                    seq = attn_seq(a, s);
+                    if (seq.q > 0) break;
+                }
             }
         }
         return true;
@@ -259,8 +261,8 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-constexpr float kAttnRefDrop = 8.0f;    // the reference lies this far under the maximum it was set by
-constexpr float kAttnRefMove = 11.0f;   // and moves when a score is this far above it
+constexpr float kAttnRefDrop = 2.0f;    // the reference lies this far under the maximum it was set by
+constexpr float kAttnRefMove = 12.0f;   // and moves when a score is this far above it
 constexpr float kAttnVRatio = 8.0f;     // the v_scale reference moves when a page's scale is this many times it
 constexpr float kLn2 = 0.69314718055994531f;
 
@@ -311,8 +313,9 @@ template <int D, bool SPLIT> struct DecCfg {
     static constexpr int kBarOff = kInfoOff + kStages * 16;
     static constexpr int kStatOff = kBarOff + kStages * 16;
     static constexpr int kRowOff = kStatOff + kAttnWarps * 16 * 8 + kAttnWarps * 16;
-    static constexpr int kPlanOff = (kRowOff + 16 * 16 + 127) / 128 * 128;
+    static constexpr int kPlanOff = kRowOff + 16 * 16;
     static constexpr int kSmem = kPlanOff + int(sizeof(AttnPlan)) + 1024;
+    static_assert(kQOff >= (kAttnMaxSeqs + 1) * 4, "the plan's scratch lies in the ring");
 };
 static_assert(DecCfg<256, true>::kSmem <= 227 * 1024 && DecCfg<256, false>::kSmem <= 227 * 1024 &&
                   DecCfg<128, true>::kSmem <= 227 * 1024 && DecCfg<128, false>::kSmem <= 227 * 1024,
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
     }
     pdl_wait();
     pdl_launch_dependents();
-    attn_make_plan<kRows, kAttnTile>(a, plan);
+    attn_make_plan<kRows, kAttnTile>(a, plan, reinterpret_cast<int *>(smem));
     AttnWalk<kRows, kAttnTile> walk(a, plan);
     AttnUnit u;
     const int lb = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;

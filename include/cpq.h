@@ -442,7 +442,7 @@ cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *const *x, cpq_
 
 /* The cache: a pool of pages of `block` tokens (16, 32, 64 or 128). A page
  * holds for each kv head block x head_dim codes and one scale, for K and for V;
- * a code c stands for c * scale. k, v: [n_pages][n_head_kv][block][head_dim]
+ * a code c stands for c * scale (scales are not negative). k, v: [n_pages][n_head_kv][block][head_dim]
  * bytes, 128-byte aligned; scales: [n_pages][n_head_kv]. head_dim 128 or 256.
  * Token slot = page * block + place in the page. The pool needs no
  * initialisation. */
