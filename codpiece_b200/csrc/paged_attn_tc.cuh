@@ -14,10 +14,12 @@
 // needs 64 (a 1024-token chunk behind 16k keys: 715 us).
 //
 // Tensor memory (512 columns): O, fp32 [128][D]; two buffers of S, fp32
-// [128][128], in which P takes its scores' place (per 32 keys 16 columns of
-// first fp16 terms, 16 of second ones). Shared memory, all with the 128-byte
+// [128][128], in which P takes its scores' place (per 16 keys 8 columns of first
+// fp16 terms, 8 of second ones). Shared memory, all with the 128-byte
 // swizzle: Q [128][D] (first, then second terms) as D / 64 blocks of 128 rows x
-// 128 bytes; K [128 keys][D] in the same blocks, one stage; V in stages of 32
+// 128 bytes; K [128 keys][D] in the same blocks, each filled and released on its
+// own (a whole K at a time left the conversion idle during the first product and
+// the tensor core during the conversion: 5700 cycles per key tile); V in stages of 32
 // keys (four; two beside fp32 q) as D / 64 blocks of 32 rows x 128 bytes. K is the
 // K-major operand of the first product (N = keys, K = dims), V the MN-major
 // operand of the second (N = dims, K = keys): the same row layout, so both come
@@ -25,18 +27,19 @@
 //
 //   warp 0       one lane issues the MMAs: per tile i S(i + 1), then P(i) V. S(i + 1)
 //                waits for P(i - 1) V, whose P lies in its buffer, and is made while
-//                the softmax of tile i runs; K's stage is refilled during P(i) V
+//                the softmax of tile i runs
 //   warp 1       the key tiles' cache rows and page scales, some tiles ahead
 //   warps 4-11   softmax: a query row is a lane of tensor memory, its first 64 keys
 //                belong to a thread of warps 4-7, the others to one of warps 8-11,
 //                which exchange their maxima through shared memory. Scores are read
-//                twice, 32 at a time (maxima, then exponentials), which keeps 20 warps
-//                within the register file. They also load Q, rescale O when a
+//                twice, 32 and then 16 at a time (maxima, exponentials), which keeps 28
+//                warps within the register file. They also load Q, rescale O when a
 //                reference moves, and write the unit's rows out, half of the columns
 //                each
-//   warps 12-15  conversion of K, warps 16-19 of V, the same code, in jobs of 32 keys:
-//                16 bytes of codes per load, two jobs in registers; keys that are not
-//                there become zeros
+//   warps 12-19  conversion of K, in jobs of a 64-dim block, warps 20-27 of V, in jobs
+//                of 32 keys, the same code, two sets of four warps that take turns
+//                (a job takes some 1200 cycles, half of them latency): 16 bytes of codes
+//                per load, two jobs in registers; keys that are not there become zeros
 //
 // The roles' inner loops are kept short: unrolled all the way, with variants for
 // masked tiles and K and V apart, the warps waited for instructions more than
@@ -55,8 +58,8 @@ constexpr int kTaRows = 128;
 constexpr int kTaTile = 128;
 constexpr int kTaHalf = 64;       // keys of a conversion job, a softmax thread
 constexpr int kTaQuarter = 32;    // keys of a V stage
-constexpr int kTaThreads = 640;
-constexpr int kTaConvWarps = 8;
+constexpr int kTaThreads = 896;
+constexpr int kTaConvWarps = 16;
 constexpr int kTaSoftWarps = 8;
 constexpr int kTaInfo = 4;        // key tiles looked up ahead
 static_assert(kTaInfo == 4, "warp 1 looks up four tiles at a time");
@@ -78,7 +81,7 @@ template <int D, bool SPLIT> struct TaCfg {
     static constexpr int kMaxOff = kQOff + (SPLIT ? 2 : 1) * kQ;   // float [2][2][128], used in turns
     static constexpr int kInfoOff = kMaxOff + 4 * kTaRows * 4;
     static constexpr int kBarOff = kInfoOff + kTaInfo * int(sizeof(TaInfo));
-    static constexpr int kBars = 2 * kTaInfo + 2 + 8 + 7;
+    static constexpr int kBars = 2 * kTaInfo + 16 + 7;
     static constexpr int kPlanOff = kBarOff + kBars * 8;
     static constexpr int kSmem = kPlanOff + int(sizeof(AttnPlan)) + 12;
     // tensor memory columns
@@ -137,6 +140,13 @@ __device__ __forceinline__ void tc_mma1_ts(uint32_t d_tmem, uint32_t a_tmem, uin
 }
 __device__ __forceinline__ void tc_commit1(uint64_t *bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// 8 columns of this thread's lane, without waiting for completion.
+__device__ __forceinline__ void tmem_st8_async(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 
 // 16 columns, load and wait in one statement.
@@ -279,8 +289,8 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
     TaInfo *info = reinterpret_cast<TaInfo *>(smem + C::kInfoOff);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::kBarOff);
     uint64_t *info_full = bars, *info_empty = bars + kTaInfo;
-    uint64_t *k_full = bars + 2 * kTaInfo, *k_empty = k_full + 1, *v_full = k_full + 2, *v_empty = k_full + 6;
-    uint64_t *q_full = k_full + 10, *s_full = q_full + 1, *p_full = q_full + 3, *pv_done = q_full + 5, *stopped = q_full + 6;
+    uint64_t *k_full = bars + 2 * kTaInfo, *k_empty = k_full + 4, *v_full = k_full + 8, *v_empty = k_full + 12;
+    uint64_t *q_full = k_full + 16, *s_full = q_full + 1, *p_full = q_full + 3, *pv_done = q_full + 5, *stopped = q_full + 6;
     AttnPlan &plan = *reinterpret_cast<AttnPlan *>(smem + C::kPlanOff);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + C::kPlanOff + sizeof(AttnPlan));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -291,10 +301,10 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             mbar_init(&info_full[i], 1);
             mbar_init(&info_empty[i], kTaConvWarps + kTaSoftWarps);
         }
-        mbar_init(k_full, 2 * kTaConvWarps);  // half of the warps, four jobs
-        mbar_init(k_empty, 1);
         for (int i = 0; i < 4; i++) {
-            mbar_init(&v_full[i], kTaConvWarps / 2);
+            mbar_init(&k_full[i], kTaConvWarps / 4);  // the warps of a set
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], kTaConvWarps / 4);
             mbar_init(&v_empty[i], 1);
         }
         mbar_init(q_full, kTaSoftWarps);
@@ -334,19 +344,21 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             const uint32_t v_lo = desc_lo(smem_addr(sV), C::kVBlock);
             // S = Q K(gi)^T; fresh: the unit's first tile, or its second (the buffer's last P V has been waited for)
             auto scores = [&](int gi, bool fresh) {
-                if (!tc_wait(k_full, uint32_t(gi) & 1u, abort_flag)) return false;
                 if (!fresh && !tc_wait(pv_done, uint32_t(gi - 2) & 1u, abort_flag)) return false;
-                tc_fence_after();
                 const uint32_t s = tmem + C::kColS + uint32_t(kTaTile) * uint32_t(gi & 1);
 #pragma unroll
-                for (int x = 0; x < (SPLIT ? 2 : 1) * (D / 16); x++) {
-                    const int t = x / (D / 16), ks = x % (D / 16);
-                    const uint32_t at = uint32_t((ks >> 2) * (C::kBlock / 16) + 2 * (ks & 3));
-                    if (x == 0) tc_mma1_ss<false>(s, q_lo, k_lo, idesc_s);
-                    else tc_mma1_ss<true>(s, q_lo + uint32_t(t * (C::kQ / 16)) + at, k_lo + at, idesc_s);
+                for (int b = 0; b < D / 64; b++) {
+                    if (!tc_wait(&k_full[b], uint32_t(gi) & 1u, abort_flag)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = 0; x < (SPLIT ? 8 : 4); x++) {
+                        const uint32_t at = uint32_t(b * (C::kBlock / 16) + 2 * (x & 3));
+                        if (b == 0 && x == 0) tc_mma1_ss<false>(s, q_lo, k_lo, idesc_s);
+                        else tc_mma1_ss<true>(s, q_lo + uint32_t((x >> 2) * (C::kQ / 16)) + at, k_lo + at, idesc_s);
+                    }
+                    issued = true;
+                    tc_commit1(&k_empty[b]);
                 }
-                issued = true;
-                tc_commit1(k_empty);
                 tc_commit1(&s_full[gi & 1]);
                 return true;
             };
@@ -361,7 +373,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 else tc_mma1_ts<true>(tmem + C::kColO, p, v, idesc_o);
 #pragma unroll
                 for (int x = 1; x < (SPLIT ? 4 : 2); x++)
-                    tc_mma1_ts<true>(tmem + C::kColO, p + 16u * uint32_t(x >> 1) + 8u * uint32_t(x & 1), v + 128u * uint32_t(x & 1), idesc_o);
+                    tc_mma1_ts<true>(tmem + C::kColO, p + 8u * uint32_t(x >> 1) + 16u * uint32_t(x & 1), v + 128u * uint32_t(x & 1), idesc_o);
                 tc_commit1(&v_empty[st]);
                 return true;
             };
@@ -423,58 +435,72 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
         }
         __syncwarp();
     } else if (warp >= 12) {
-        // ---- conversion: keys 8 w .. 8 w + 7 of every job; job j: keys 32 (j & 3) .. of tile j >> 2 ----
+        // ---- conversion ----
+        // V: job j is the keys 32 (j & 3) .. of tile j / 4, a warp's part 8 keys, all dims.
+        // K: job j is the 64-dim block j % (D / 64) of tile j / (D / 64), a warp's part 32 keys.
+        // Load i of a lane: 16 dims of key key_in + step * i.
         const int w = warp & 3;
-        const bool is_v = warp >= 16;
-        constexpr int kLanes = D / 16, kPer = 32 / kLanes, kLoads = 8 / kPer;  // lanes per key, keys per load, loads
-        const int key_in = 8 * w + lane / kLanes, d0 = (lane % kLanes) * 16;   // of load 0
-        // where the lane's 16 values go: two 16-byte units of its 64-dim block. Odd blocks store their second
+        const int set = (warp >> 2) - 3 & 1;
+        const bool is_v = warp >= 20;
+        constexpr int kLoads = 4, kLanes = D / 16, kVLoads = kLanes / 4;  // (V has two loads at D = 128)
+        const int per_tile = is_v ? 4 : D / 64, step = is_v ? 32 / kLanes : 8;
+        const int key_in = is_v ? 8 * w + lane / kLanes : 32 * w + (lane >> 2);
+        const int d0 = is_v ? (lane % kLanes) * 16 : (lane & 3) * 16;
+        // where the lane's 16 values go: two 16-byte units of a 64-dim block. Odd blocks store their second
         // unit first, so that a quarter warp's eight stores fall into eight bank groups.
         const int blk = d0 >> 6, unit = (d0 & 63) >> 3, swap = blk & 1;
         const uint8_t *const codes = (is_v ? a.v : a.k) + (key_in & 15) * D + d0;
-        uint8_t *const dst0 = (is_v ? sV + blk * C::kVBlock : sK + blk * C::kBlock) + key_in * 128;
-        const int n_jobs = 4 * n_tiles;
+        uint8_t *const dst0 = (is_v ? sV + blk * C::kVBlock : sK) + key_in * 128;
+        const int n_jobs = per_tile * n_tiles;
         auto load = [&](int j, uint4 (&x)[kLoads]) {
             if (j >= n_jobs) return true;
-            const int tile = j >> 2, slot = tile % kTaInfo;
+            const int tile = j / per_tile, part = j - tile * per_tile, slot = tile % kTaInfo;
             if (!tc_wait(&info_full[slot], uint32_t(tile / kTaInfo) & 1u, abort_flag)) return false;
-            const int keys = info[slot].keys - kTaQuarter * (j & 3);
-            const int row = info[slot].row[2 * (j & 3) + (w >> 1)];  // the warp's keys lie in one group of 16
-            const uint8_t *at = codes + int64_t(row) * D;
+            const int keys = info[slot].keys - (is_v ? kTaQuarter * part : 0) - key_in;
+            // the lane's keys lie in one group of 16 (V), or two (K)
+            const int grp = is_v ? 2 * part + (w >> 1) : 2 * w;
+            const int row0 = info[slot].row[grp], row1 = is_v ? row0 : info[slot].row[grp + 1] - 16;
+            const uint8_t *at = codes + (is_v ? 0 : 64 * part);
 #pragma unroll
-            for (int i = 0; i < kLoads; i++) x[i] = ldg_codes(at + kPer * i * D, row >= 0 && key_in + kPer * i < keys);
-            if ((j & 3) == 3) {  // the tile's last job
+            for (int i = 0; i < kLoads; i++) {
+                const int row = i < 2 ? row0 : row1;
+                const bool there = row >= (i < 2 || is_v ? 0 : -16) && step * i < keys && (i < kVLoads || !is_v);
+                x[i] = ldg_codes(at + (int64_t(row) + step * i) * D, there);
+            }
+            if (part + 2 >= per_tile) {  // the set's last job of the tile
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&info_empty[slot]);
             }
             return true;
         };
         auto run = [&](int j, uint4 (&x)[kLoads]) {  // job j, whose codes are in x
-            const int st = is_v ? j % C::kVStages : 0, use = is_v ? j / C::kVStages : j >> 2;
-            if (!tc_wait(is_v ? &v_empty[st] : k_empty, (uint32_t(use) & 1u) ^ 1u, abort_flag)) return false;
-            uint8_t *const dst = dst0 + (is_v ? st * C::kV : (j & 3) * (kTaQuarter * 128));
+            if (j >= n_jobs) return true;
+            const int st = is_v ? j % C::kVStages : j % (D / 64), use = is_v ? j / C::kVStages : j / (D / 64);
+            if (!tc_wait((is_v ? v_empty : k_empty) + st, (uint32_t(use) & 1u) ^ 1u, abort_flag)) return false;
+            uint8_t *const dst = dst0 + st * (is_v ? C::kV : C::kBlock);
 #pragma unroll
             for (int i = 0; i < kLoads; i++) {
+                if (i >= kVLoads && is_v) break;
                 uint32_t h[8];
                 codes_h2<FMT>(x[i].x, h[0], h[1]);
                 codes_h2<FMT>(x[i].y, h[2], h[3]);
                 codes_h2<FMT>(x[i].z, h[4], h[5]);
                 codes_h2<FMT>(x[i].w, h[6], h[7]);
                 const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-                const int k7 = (key_in + kPer * i) & 7;
-                uint8_t *at = dst + kPer * i * 128;
+                const int k7 = (key_in + step * i) & 7;
+                uint8_t *at = dst + step * i * 128;
                 *reinterpret_cast<uint4 *>(at + (((unit + swap) ^ k7) << 4)) = swap ? hi : lo;
                 *reinterpret_cast<uint4 *>(at + (((unit + (swap ^ 1)) ^ k7) << 4)) = swap ? lo : hi;
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(is_v ? &v_full[st] : k_full);
-            return load(j + 2, x);
+            if (lane == 0) mbar_arrive((is_v ? v_full : k_full) + st);
+            return load(j + 4, x);
         };
         uint4 x0[kLoads], x1[kLoads];
-        bool ok = load(0, x0) && load(1, x1);
+        bool ok = load(set, x0) && load(set + 2, x1);
 #pragma unroll 1
-        for (int j = 0; ok && j < n_jobs; j += 2) ok = run(j, x0) && run(j + 1, x1);
+        for (int j = set; ok && j < n_jobs; j += 4) ok = run(j, x0) && run(j + 2, x1);
         __syncwarp();
     } else {
         // ---- softmax: row = lane of tensor memory, 64 of the tile's keys per thread ----
@@ -608,30 +634,26 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 const uint64_t nbase = f2_pack(-base, -base);
                 uint64_t part[2] = {0, 0};  // (two zeros each)
 #pragma unroll 1
-                for (int c = 0; c < 2; c++) {
-                    float z[32];
-                    tmem_ld32_wait(ts + 32u * uint32_t(c), z);
-                    uint32_t hi[16], lo[16];
+                for (int c = 0; c < 4; c++) {
+                    uint32_t z[16], hi[8], lo[8];
+                    tmem_ld16_wait(ts + 16u * uint32_t(c), z);
+                    const float kf = ta_factor(in.ks[4 * hf + c] * qf), r = in.vs[4 * hf + c] * vinv;
+                    const uint64_t kf2 = f2_pack(kf, kf), r2 = f2_pack(r, r);
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float kf = ta_factor(in.ks[4 * hf + 2 * c + h] * qf), r = in.vs[4 * hf + 2 * c + h] * vinv;
-                        const uint64_t kf2 = f2_pack(kf, kf), r2 = f2_pack(r, r);
-#pragma unroll
-                        for (int i = 8 * h; i < 8 * h + 8; i++) {
-                            float p0, p1;
-                            f2_unpack(f2_fma(f2_pack(z[2 * i], z[2 * i + 1]), kf2, nbase), p0, p1);
-                            uint64_t p = f2_pack(ex2(p0), ex2(p1));
-                            part[i & 1] = f2_add(part[i & 1], p);
-                            f2_unpack(f2_mul(p, r2), p0, p1);
-                            hi[i] = pack_h2(p0, p1);
-                            if constexpr (SPLIT) {
-                                const float2 f = __half22float2(u32_half2(hi[i]));
-                                lo[i] = pack_h2(p0 - f.x, p1 - f.y);
-                            }
+                    for (int i = 0; i < 8; i++) {
+                        float p0, p1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), kf2, nbase), p0, p1);
+                        const uint64_t p = f2_pack(ex2(p0), ex2(p1));
+                        part[i & 1] = f2_add(part[i & 1], p);
+                        f2_unpack(f2_mul(p, r2), p0, p1);
+                        hi[i] = pack_h2(p0, p1);
+                        if constexpr (SPLIT) {
+                            const float2 f = __half22float2(u32_half2(hi[i]));
+                            lo[i] = pack_h2(p0 - f.x, p1 - f.y);
                         }
                     }
-                    tmem_st16_async(ts + 32u * uint32_t(c), hi);
-                    if constexpr (SPLIT) tmem_st16_async(ts + 32u * uint32_t(c) + 16u, lo);
+                    tmem_st8_async(ts + 16u * uint32_t(c), hi);
+                    if constexpr (SPLIT) tmem_st8_async(ts + 16u * uint32_t(c) + 8u, lo);
                 }
                 {
                     float s0, s1;
