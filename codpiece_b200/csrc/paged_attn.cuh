@@ -21,9 +21,11 @@
 //
 // Work. The query rows of one kv head and sequence, (token, head of the group)
 // in that order, form row tiles of kRows rows; a unit is (sequence, row tile,
-// kv head) with its visible keys in tiles. All units' tiles in a row form one
-// range that is cut into equal shares, one per CTA: ragged batches, causal
-// triangles and one long sequence balance alike. A unit that is cut leaves
+// kv head) with its visible keys in tiles. All units in a row, each as long as
+// its tiles plus what beginning it costs in tiles (START), form one range that is
+// cut into equal shares, one per CTA: ragged batches, causal triangles and one
+// long sequence balance alike (without START a CTA could draw a dozen units of
+// one tile: 32 ragged requests took 231 us, equal ones 127). A unit that is cut leaves
 // partial sums, softmax reference and row sums in the workspace, which
 // attn_combine_kernel joins in key order (same split, same result).
 #pragma once
@@ -39,7 +41,7 @@ namespace cpq {
 constexpr int kAttnMaxSeqs = 1024;
 
 struct alignas(64) AttnArgs {
-    CUtensorMap tmap_k, tmap_v;  // codes as [n_pages * n_head_kv * block][D] bytes, box 128 x min(block, 32)
+    CUtensorMap tmap_k, tmap_v;  // codes as [D / 128][n_pages * n_head_kv * block][128] bytes, box 128 x min(block, 32) x D / 128
     const uint8_t *k, *v;
     const float *k_scale, *v_scale;
     int64_t n_pages;
@@ -56,7 +58,7 @@ struct alignas(64) AttnArgs {
     int64_t table_stride;
     int max_blocks, causal;
     float scale_log2;            // softmax scale * log2(e)
-    int min_tiles;               // a CTA's share is at least this many tiles
+    int min_share;               // a CTA's share is at least this many places
     // workspace: two slots per CTA (the unit that ends in it, the unit that begins in it)
     float *part_o;               // [slot][kRows][D]
     float2 *part_ml;             // [slot][kRows]: softmax reference, row sum
@@ -86,21 +88,21 @@ __device__ __forceinline__ int attn_kv_end(const AttnSeq &s, int r, int rows, in
 
 __device__ __forceinline__ int attn_row_tiles(const AttnSeq &s, int rows, int group) { return (s.q * group + rows - 1) / rows; }
 
-// Where a CTA's share of the tiles begins.
+// Where a CTA's share begins.
 struct AttnPlan {
-    int s, r, h, tile, left;  // unit and tile, and the share's tiles
+    int s, r, h, at, left;  // unit, place in it (START places, then its tiles), and the share's places
 };
 
 // Fills the plan (all threads of the CTA; barriers inside). through: scratch of
 // kAttnMaxSeqs + 1 ints, free again afterwards. A unit with no visible key
 // counts one tile, so that some CTA writes its rows. Also marks the CTA's
 // workspace slots unused, before any is written.
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, int START>
 __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, int *through) {
     if (threadIdx.x < 2) a.part_hdr[2 * blockIdx.x + threadIdx.x] = make_int4(0, 0, 0, 0);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n_warps = blockDim.x >> 5;
-    auto tiles = [&](const AttnSeq &s, int r) {
-        return max(1, (attn_kv_end(s, r, ROWS, a.group, a.causal) + TILE - 1) / TILE);
+    auto places = [&](const AttnSeq &s, int r) {
+        return START + max(1, (attn_kv_end(s, r, ROWS, a.group, a.causal) + TILE - 1) / TILE);
     };
     for (int s = tid; s < a.n_seqs; s += blockDim.x) {
         const AttnSeq q = attn_seq(a, s);
@@ -108,7 +110,7 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, i
         int w = -1;  // many row tiles: counted by a warp below
         if (n <= 4) {
             w = 0;
-            for (int r = 0; r < n; r++) w += tiles(q, r);
+            for (int r = 0; r < n; r++) w += places(q, r);
         }
         through[s + 1] = w < 0 ? -1 : w * a.hkv;
     }
@@ -118,7 +120,7 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, i
         const AttnSeq q = attn_seq(a, s);
         const int n = attn_row_tiles(q, ROWS, a.group);
         int w = 0;
-        for (int r = lane; r < n; r += 32) w += tiles(q, r);
+        for (int r = lane; r < n; r += 32) w += places(q, r);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
         __syncwarp();
@@ -139,13 +141,13 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, i
         }
         if (lane == 0) through[0] = 0;
         __syncwarp();
-        const int n_cta = max(1, min(int(gridDim.x), sum / a.min_tiles));
+        const int n_cta = max(1, min(int(gridDim.x), sum / a.min_share));
         const int c = blockIdx.x;
         const int x0 = c < n_cta ? int(int64_t(sum) * c / n_cta) : sum;
         const int x1 = c < n_cta ? int(int64_t(sum) * (c + 1) / n_cta) : sum;
-        int s = 0, r = 0, h = 0, tile = 0;
+        int s = 0, r = 0, h = 0, at = 0;
         if (x1 > x0) {
-            int lo = 0, hi = a.n_seqs;  // the last sequence that begins at or before x0 (and so has tiles there)
+            int lo = 0, hi = a.n_seqs;  // the last sequence that begins at or before x0 (and so has places there)
             while (hi - lo > 1) {
                 const int mid = (lo + hi) / 2;
                 if (through[mid] <= x0) lo = mid;
@@ -156,7 +158,7 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, i
             const AttnSeq q = attn_seq(a, s);
             const int n = attn_row_tiles(q, ROWS, a.group);
             for (int r0 = 0; r0 < n; r0 += 32) {  // row tiles in order, each with its hkv units
-                const int mine = r0 + lane < n ? tiles(q, r0 + lane) * a.hkv : 0;
+                const int mine = r0 + lane < n ? places(q, r0 + lane) * a.hkv : 0;
                 int w = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -165,18 +167,18 @@ __device__ __forceinline__ void attn_make_plan(const AttnArgs &a, AttnPlan &p, i
                 }
                 const unsigned after = __ballot_sync(0xffffffffu, w > rem);
                 if (after) {
-                    const int at = __ffs(int(after)) - 1;
-                    const int before = __shfl_sync(0xffffffffu, w - mine, at);
-                    const int per = __shfl_sync(0xffffffffu, mine, at) / a.hkv;
-                    r = r0 + at;
+                    const int i = __ffs(int(after)) - 1;
+                    const int before = __shfl_sync(0xffffffffu, w - mine, i);
+                    const int per = __shfl_sync(0xffffffffu, mine, i) / a.hkv;
+                    r = r0 + i;
                     h = (rem - before) / per;
-                    tile = (rem - before) - h * per;
+                    at = (rem - before) - h * per;
                     break;
                 }
                 rem -= __shfl_sync(0xffffffffu, w, 31);
             }
         }
-        if (lane == 0) p.s = s, p.r = r, p.h = h, p.tile = tile, p.left = x1 - x0;
+        if (lane == 0) p.s = s, p.r = r, p.h = h, p.at = at, p.left = x1 - x0;
     }
     __syncthreads();
 }
@@ -189,12 +191,12 @@ struct AttnUnit {
 };
 
 // Walks the CTA's units; every role of the CTA does so by itself.
-template <int ROWS, int TILE>
+template <int ROWS, int TILE, int START>
 struct AttnWalk {
     const AttnArgs &a;
-    int s, r, h, tile, left;
+    int s, r, h, at, left;
     AttnSeq seq;
-    __device__ AttnWalk(const AttnArgs &a_, const AttnPlan &p) : a(a_), s(p.s), r(p.r), h(p.h), tile(p.tile), left(p.left) {
+    __device__ AttnWalk(const AttnArgs &a_, const AttnPlan &p) : a(a_), s(p.s), r(p.r), h(p.h), at(p.at), left(p.left) {
         if (left > 0) seq = attn_seq(a, s);
     }
     __device__ bool next(AttnUnit &u) {
@@ -203,10 +205,12 @@ struct AttnWalk {
         u.seq = seq;
         u.kv_end = attn_kv_end(seq, r, ROWS, a.group, a.causal);
         u.n = max(1, (u.kv_end + TILE - 1) / TILE);
-        u.t0 = tile;
-        u.t1 = min(u.n, tile + left);
-        left -= u.t1 - u.t0;
-        tile = 0;
+        const int to = min(START + u.n, at + left);
+        u.t0 = max(0, at - START);
+        u.t1 = max(0, to - START);
+        left -= to - at;
+        at = 0;
+        if (u.t1 == u.t0) return false;  // the share ends before the unit's first tile
         if (++h == a.hkv) {
             h = 0;
             if (++r == attn_row_tiles(seq, ROWS, a.group)) {
@@ -273,15 +277,16 @@ __device__ __forceinline__ float attn_lse(float ref, float sum) {
 
 // ---- few query rows: mma.sync tiles, one key tile per warp -------------------------
 //
-// Decode reads the cache once and does little with it, so the kernel is built
-// around the copy: one CTA per SM, a producer warp that keeps a ring of 32-key
-// tiles (K and V codes, TMA boxes of 128 bytes x up to 32 keys, 128-byte
-// swizzle) in flight, and eight warps that each take every eighth tile with
-// their own softmax state and output accumulators, so that nothing but the
-// end of a unit makes warps wait for one another. m16n8k16 fp16 MMAs: 16 rows
-// of 16-bit q, or 8 rows of fp32 q with the first terms in rows 0-7 and the
-// second terms in rows 8-15 of the same MMA (they meet in one thread, lanes
-// of row g hold both), so fp32 costs no extra MMA.
+// Decode reads the cache once and does little with it. One CTA per SM; each of
+// its warps takes every kWarps-th 32-key tile with its own softmax state, output
+// accumulators and copies (K two tiles ahead, V one, TMA boxes of 128 bytes x
+// up to 32 keys, 128-byte swizzle), so that nothing but the end of a unit makes
+// warps wait for one another. m16n8k16 fp16 MMAs: 16 rows of 16-bit q, or 8 rows
+// of fp32 q with the first terms in rows 0-7 and the second terms in rows 8-15
+// of the same MMA (they meet in one thread, lanes of row g hold both), so fp32
+// costs no extra MMA. A warp copies for itself because a ninth warp would cost
+// the others a quarter of their registers (warps are allotted in fours): with
+// one, the accumulators of D = 256 spilled.
 //
 // Operand order. A key tile's codes go from shared memory to the MMA's B
 // registers without a transpose:
@@ -295,31 +300,35 @@ __device__ __forceinline__ float attn_lse(float ref, float sum) {
 // loads touch eight different bank groups in both.
 
 constexpr int kAttnTile = 32;
-constexpr int kAttnWarps = 8;
-constexpr int kAttnThreads = 32 * (kAttnWarps + 1);
 
 template <int D, bool SPLIT> struct DecCfg {
     static constexpr int kRows = SPLIT ? 8 : 16;
-    static constexpr int kHalfBytes = kAttnTile * D;              // K or V codes of a tile
-    static constexpr int kStageBytes = 2 * kHalfBytes;
-    static constexpr int kStages = D == 256 ? (SPLIT ? 10 : 8) : (SPLIT ? 20 : 18);
-    static constexpr int kRedBytes = 4 * kRows * D * 4;          // four warps' accumulators
-    static constexpr int kQBytes = D / 16 * 512;
-    static constexpr int kQOff = kStages * kStageBytes;
-    static constexpr int kRedOff = kQOff + kQBytes;
-    static constexpr int kSmallOff = kRedOff + kRedBytes;
-    // small: stage info float4, full/empty barriers, stats (ref, sum, v reference) per warp and row, row factors
-    static constexpr int kInfoOff = kSmallOff;
-    static constexpr int kBarOff = kInfoOff + kStages * 16;
-    static constexpr int kStatOff = kBarOff + kStages * 16;
-    static constexpr int kRowOff = kStatOff + kAttnWarps * 16 * 8 + kAttnWarps * 16;
-    static constexpr int kPlanOff = kRowOff + 16 * 16;
+    static constexpr int kWarps = D == 256 ? 8 : 12;             // D = 256: 255 registers, D = 128: 168
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kStart = kWarps;                        // beginning a unit takes about as long as a tile per warp
+    static constexpr int kCodes = kAttnTile * D;                 // K or V codes of a tile
+    static constexpr int kVOff = kWarps * 2 * kCodes;            // K: two slots per warp; V: one
+    static constexpr int kQOff = kVOff + kWarps * kCodes;
+    static constexpr int kRedBytes = 4 * kRows * D * 4;          // four warps' accumulators, in V's place
+    static constexpr int kBarOff = kQOff + D / 16 * 512;
+    // stats (reference, sum) per warp and row, v reference per warp, row factors
+    static constexpr int kStatOff = kBarOff + kWarps * 3 * 8;
+    static constexpr int kVStatOff = kStatOff + kWarps * 16 * 8;
+    static constexpr int kRowOff = kVStatOff + kWarps * 4;
+    static constexpr int kPlanOff = kRowOff + 16 * 4;
     static constexpr int kSmem = kPlanOff + int(sizeof(AttnPlan)) + 1024;
-    static_assert(kQOff >= (kAttnMaxSeqs + 1) * 4, "the plan's scratch lies in the ring");
+    static_assert(kRedBytes <= kWarps * kCodes, "the accumulators fit in V's place");
+    static_assert(kVOff >= (kAttnMaxSeqs + 1) * 4, "the plan's scratch lies in K's place");
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
-static_assert(DecCfg<256, true>::kSmem <= 227 * 1024 && DecCfg<256, false>::kSmem <= 227 * 1024 &&
-                  DecCfg<128, true>::kSmem <= 227 * 1024 && DecCfg<128, false>::kSmem <= 227 * 1024,
-              "shared memory");
+
+// 3-D tiled TMA load (no multicast) completing as transaction bytes on `bar`.
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -330,104 +339,99 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) { return h2u(__floats2half2_rn(a, b)); }
 
-__device__ __forceinline__ void dec_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kAttnWarps) : "memory"); }
+// Pages and scales of up to 32 of a warp's tiles, one per lane (two pages with
+// 16-token pages); a page that is not there is -1.
+struct DecInfo {
+    int page[2];
+    float ks[2], vs[2];
+};
 
 template <int D, int FMT, bool SPLIT>
-__global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_kernel(const __grid_constant__ AttnArgs a) {
     using C = DecCfg<D, SPLIT>;
-    constexpr int kRows = C::kRows, NA = D / 128;  // 128-byte atoms per key
+    constexpr int kRows = C::kRows, NA = D / 128, W = C::kWarps;  // NA: 128-byte atoms per key
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint4 *sq = reinterpret_cast<uint4 *>(smem + C::kQOff);
-    float *red = reinterpret_cast<float *>(smem + C::kRedOff);
-    float4 *info = reinterpret_cast<float4 *>(smem + C::kInfoOff);  // k_scale, v_scale of keys 0-15 and 16-31 (NaN: no page)
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff), *empty = full + C::kStages;
+    float *red = reinterpret_cast<float *>(smem + C::kVOff);
     float2 *stat = reinterpret_cast<float2 *>(smem + C::kStatOff);  // [warp][16 rows]: reference, sum
-    float *vstat = reinterpret_cast<float *>(stat + kAttnWarps * 16);
+    float *vstat = reinterpret_cast<float *>(smem + C::kVStatOff);
     float *rowf = reinterpret_cast<float *>(smem + C::kRowOff);     // [row]: 2^-shift of its q
     AttnPlan &plan = *reinterpret_cast<AttnPlan *>(smem + C::kPlanOff);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t *const my_k = smem + warp * 2 * C::kCodes, *const my_v = smem + C::kVOff + warp * C::kCodes;
+    uint64_t *const k_bar = reinterpret_cast<uint64_t *>(smem + C::kBarOff) + 3 * warp, *const v_bar = k_bar + 2;
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < C::kStages; i++) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
+    if (lane == 0) {
+        for (int i = 0; i < 3; i++) mbar_init(&k_bar[i], 1);
         fence_mbar_init();
     }
     pdl_wait();
     pdl_launch_dependents();
-    attn_make_plan<kRows, kAttnTile>(a, plan, reinterpret_cast<int *>(smem));
-    AttnWalk<kRows, kAttnTile> walk(a, plan);
+    attn_make_plan<kRows, kAttnTile, C::kStart>(a, plan, reinterpret_cast<int *>(smem));
+    fence_proxy_async_smem();  // the plan's scratch before the copies into its place
+    AttnWalk<kRows, kAttnTile, C::kStart> walk(a, plan);
     AttnUnit u;
     const int lb = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
+    const int pages = a.block == 16 ? 2 : 1, box = a.block < kAttnTile ? a.block : kAttnTile;
 
-    if (warp == kAttnWarps) {
-        // ---- producer: 32 tiles' pages and scales at a time, one tile per lane ----
-        const int pages = a.block == 16 ? 2 : 1, box = a.block < kAttnTile ? a.block : kAttnTile;
-        int g = 0;  // tiles issued
-        bool ok = true;
-        while (ok && walk.next(u)) {
-            for (int b0 = u.t0; b0 < u.t1 && ok; b0 += 32) {
-                int page[2] = {-1, -1};
-                float ks[2], vs[2];
-                const float nan = __int_as_float(0x7fffffff);
+    // This warp's tiles of a unit: its i-th is unit tile t_first + W i (tile x of the CTA, counted over
+    // units, goes to warp x % W).
+    int t_first = 0, n_own = 0;
+    // lanes 0..31: tiles 32 b .. 32 b + 31 of the warp
+    auto look = [&](int b) {
+        DecInfo f;
+        const int key = (t_first + W * (32 * b + lane)) * kAttnTile;
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    ks[j] = vs[j] = nan;
-                    const int key = (b0 + lane) * kAttnTile + 16 * j;
-                    if (b0 + lane < u.t1 && key < u.kv_end && j < pages) page[j] = attn_page(a, u.s, key >> lb);
-                    if (page[j] >= 0) {
-                        ks[j] = a.k_scale[int64_t(page[j]) * a.hkv + u.h];
-                        vs[j] = a.v_scale[int64_t(page[j]) * a.hkv + u.h];
-                    }
-                }
-                if (pages == 1) ks[1] = ks[0], vs[1] = vs[0];
-                const int n = min(32, u.t1 - b0);
-                for (int i = 0; i < n; i++, g++) {
-                    const int st = g % C::kStages;
-                    const float4 f = make_float4(__shfl_sync(0xffffffffu, ks[0], i), __shfl_sync(0xffffffffu, vs[0], i),
-                                                 __shfl_sync(0xffffffffu, ks[1], i), __shfl_sync(0xffffffffu, vs[1], i));
-                    const int p0 = __shfl_sync(0xffffffffu, page[0], i), p1 = __shfl_sync(0xffffffffu, page[1], i);
-                    if (lane == 0) ok = mbar_wait_bounded(&empty[st], (uint32_t(g / C::kStages) & 1u) ^ 1u);
-                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                    if (!ok) break;
-                    if (lane == 0) {
-                        info[st] = f;
-                        const int have = (p0 >= 0) + (p1 >= 0);
-                        mbar_arrive_expect_tx(&full[st], uint32_t(have * box) * (2u * D));
-                        uint8_t *dst = smem + st * C::kStageBytes;
-                        for (int j = 0; j < pages; j++) {
-                            const int pg = j ? p1 : p0;
-                            if (pg < 0) continue;
-                            // the tile's first key inside its page
-                            const int in = j ? 0 : ((b0 + i) * kAttnTile) & (a.block - 1);
-                            const int row = (pg * a.hkv + u.h) * a.block + in;
-#pragma unroll
-                            for (int at = 0; at < NA; at++) {
-                                tma_load_2d(dst + at * (kAttnTile * 128) + j * (16 * 128), &a.tmap_k, at * 128, row, &full[st]);
-                                tma_load_2d(dst + C::kHalfBytes + at * (kAttnTile * 128) + j * (16 * 128), &a.tmap_v, at * 128, row,
-                                            &full[st]);
-                            }
-                        }
-                    }
-                }
+        for (int j = 0; j < 2; j++) {
+            f.page[j] = -1;
+            f.ks[j] = f.vs[j] = 0.0f;
+            if (32 * b + lane < n_own && key + 16 * j < u.kv_end && j < pages) f.page[j] = attn_page(a, u.s, (key + 16 * j) >> lb);
+            if (f.page[j] >= 0) {
+                f.ks[j] = a.k_scale[int64_t(f.page[j]) * a.hkv + u.h];
+                f.vs[j] = a.v_scale[int64_t(f.page[j]) * a.hkv + u.h];
             }
         }
-        // no copy may land after the CTA has left
-        if (lane == 0)
-            for (int x = g > C::kStages ? g - C::kStages : 0; x < g; x++)
-                mbar_wait_bounded(&full[x % C::kStages], uint32_t(x / C::kStages) & 1u);
-        return;
-    }
+        if (pages == 1) f.page[1] = f.page[0], f.ks[1] = f.ks[0], f.vs[1] = f.vs[0];
+        return f;
+    };
+    // copies the codes of the warp's tile i (whose info is lane i % 32's of f)
+    auto copy = [&](const DecInfo &f, int i, const CUtensorMap *map, uint8_t *dst, uint64_t *bar) {
+        const int p0 = __shfl_sync(0xffffffffu, f.page[0], i & 31), p1 = __shfl_sync(0xffffffffu, f.page[1], i & 31);
+        if (lane == 0) {
+            const int have = (p0 >= 0) + (pages == 2 && p1 >= 0);
+            mbar_arrive_expect_tx(bar, uint32_t(have * box * D));
+            const int in = pages == 2 ? 0 : ((t_first + W * i) * kAttnTile) & (a.block - 1);  // the tile's first key in its page
+            if (p0 >= 0) tma_load_3d(dst, map, 0, (p0 * a.hkv + u.h) * a.block + in, 0, bar);
+            if (pages == 2 && p1 >= 0) tma_load_3d(dst + NA * 16 * 128, map, 0, (p1 * a.hkv + u.h) * a.block, 0, bar);
+        }
+    };
+    // the byte offset of a key's 128-byte atom in a tile: [atom][key], or with 16-token pages [page][atom][key]
+    const int at_stride = box * 128, half_skip = pages == 2 ? (NA - 1) * 16 * 128 : 0;
 
-    // ---- eight warps: tile x of the CTA goes to warp x % 8 ----
-    const int gq = lane >> 2, tq = lane & 3;
-    int base = 0;       // tiles of the units before
+    DecInfo cur, nxt;   // the current and the next 32 tiles
+    int kc = 0, vc = 0; // tiles consumed over units: slots and parities
+    int base = 0;       // the CTA's tiles of the units before
     bool dead = false;  // a wait has given up: take part in barriers only
-    while (walk.next(u)) {
+    // the unit's first copies of K (V's place may still hold accumulators)
+    auto begin = [&]() {
+        const int x = ((warp - base) % W + W) % W, n = u.t1 - u.t0;
+        t_first = u.t0 + x;
+        n_own = x < n ? (n - x + W - 1) / W : 0;
+        base += n;
+        cur = look(0);
+        nxt = cur;
+        if (n_own > 0) copy(cur, 0, &a.tmap_k, my_k + (kc & 1) * C::kCodes, &k_bar[kc & 1]);
+        if (n_own > 1) copy(cur, 1, &a.tmap_k, my_k + ((kc + 1) & 1) * C::kCodes, &k_bar[(kc + 1) & 1]);
+    };
+    const int gq = lane >> 2, tq = lane & 3;
+    bool more = walk.next(u);
+    if (more) begin();
+    bool gave_up = false;
+    while (more && !gave_up) {
+        if (n_own > 0) copy(cur, 0, &a.tmap_v, my_v, v_bar);
         // q of the unit's rows, as A fragments in the K order above
-        for (int rr = warp; rr < kRows; rr += kAttnWarps) {
+        for (int rr = warp; rr < kRows; rr += W) {
             const int row = u.r * kRows + rr;
             const bool there = row < u.seq.q * a.group;
             constexpr int E = D / 32;
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                 }
             }
         }
-        dec_sync();
+        __syncthreads();
 
         constexpr int NR = SPLIT ? 1 : 2;  // real rows per lane: gq (and gq + 8)
         float o[D / 8][4];
@@ -479,27 +483,31 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
             lim[k] = a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + row / a.group + 1) : u.seq.kv;
         }
         float vref = 0.0f;
-        const int n_here = u.t1 - u.t0;
-        // every tile of the CTA has one warp: tile x of it (counted over units) goes to warp x % 8
-        for (int x = (warp - base % kAttnWarps + kAttnWarps) % kAttnWarps; x < n_here; x += kAttnWarps) {
-            const int gx = base + x, st = gx % C::kStages;
-            if (!dead && !mbar_wait_bounded(&full[st], uint32_t(gx / C::kStages) & 1u)) dead = true;
+        for (int i = 0; i < n_own; i++, kc++, vc++) {
+            if ((i & 31) == 0) {  // lanes look at the warp's next 32 tiles, long before they are needed
+                cur = nxt;
+                if (i + 32 < n_own) nxt = look(i / 32 + 1);
+            }
+            const int key0 = (t_first + W * i) * kAttnTile;
+            const bool in0 = __shfl_sync(0xffffffffu, cur.page[0], i & 31) >= 0, in1 = __shfl_sync(0xffffffffu, cur.page[1], i & 31) >= 0;
+            const float ks0 = __shfl_sync(0xffffffffu, cur.ks[0], i & 31), ks1 = __shfl_sync(0xffffffffu, cur.ks[1], i & 31);
+            const float vs0 = __shfl_sync(0xffffffffu, cur.vs[0], i & 31), vs1 = __shfl_sync(0xffffffffu, cur.vs[1], i & 31);
+            const int st = kc & 1;
+            if (!dead && !mbar_wait_bounded(&k_bar[st], uint32_t(kc >> 1) & 1u)) dead = true;
             dead = __any_sync(0xffffffffu, dead);
-            if (dead) continue;
-            const int key0 = (u.t0 + x) * kAttnTile;
-            const float4 sc = info[st];
-            const uint8_t *sk = smem + st * C::kStageBytes, *sv = sk + C::kHalfBytes;
+            if (dead) break;
+            const uint8_t *const sk = my_k + st * C::kCodes;
             float s[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.0f;
-#pragma unroll
+            for (int nt = 0; nt < 4; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll 1
             for (int at = 0; at < NA; at++) {
                 uint4 kw[4][2];
 #pragma unroll
                 for (int nt = 0; nt < 4; nt++)
 #pragma unroll
                     for (int c = 0; c < 2; c++)
-                        kw[nt][c] = *reinterpret_cast<const uint4 *>(sk + at * (kAttnTile * 128) + (8 * nt + gq) * 128 +
+                        kw[nt][c] = *reinterpret_cast<const uint4 *>(sk + at * at_stride + (nt >> 1) * half_skip + (8 * nt + gq) * 128 +
                                                                      (((2 * tq + c) ^ gq) << 4));
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -515,8 +523,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                     }
                 }
             }
-            // scores in log2, masked; a page that is not there has NaN scales
-            const bool in0 = sc.x == sc.x, in1 = sc.z == sc.z;
+            __syncwarp();
+            if (i + 2 < n_own) copy((i + 2) / 32 == i / 32 ? cur : nxt, i + 2, &a.tmap_k, my_k + st * C::kCodes, &k_bar[st]);
+            // scores in log2, masked
             float p[NR][8];
             float mx[NR];
 #pragma unroll
@@ -524,7 +533,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                 mx[k] = ninf;
 #pragma unroll
                 for (int nt = 0; nt < 4; nt++) {
-                    const float f = qf[k] * (nt < 2 ? sc.x : sc.z);
+                    const float f = qf[k] * (nt < 2 ? ks0 : ks1);
                     const bool in = nt < 2 ? in0 : in1;
 #pragma unroll
                     for (int c = 0; c < 2; c++) {
@@ -538,7 +547,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                 mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
             }
             // references: moved for the whole warp at once, seldom
-            const float vmax = fmaxf(in0 ? sc.y : 0.0f, in1 ? sc.w : 0.0f);
+            const float vmax = fmaxf(vs0, vs1);  // 0 where there is no page
             bool move = vmax > kAttnVRatio * vref;
 #pragma unroll
             for (int k = 0; k < NR; k++) move |= mx[k] > ref[k] + kAttnRefMove;
@@ -559,63 +568,68 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                     of[k] = f * vf;
                 }
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    o[i][0] *= of[0], o[i][1] *= of[0];
-                    o[i][2] *= of[NR - 1], o[i][3] *= of[NR - 1];
+                for (int n = 0; n < D / 8; n++) {
+                    o[n][0] *= of[0], o[n][1] *= of[0];
+                    o[n][2] *= of[NR - 1], o[n][3] *= of[NR - 1];
                 }
             }
-            const float r0 = in0 && vref > 0.0f ? sc.y / vref : 0.0f, r1 = in1 && vref > 0.0f ? sc.w / vref : 0.0f;
+            const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f, r0 = vs0 * vinv, r1 = vs1 * vinv;
 #pragma unroll
             for (int k = 0; k < NR; k++) {
                 const float base_ref = ref[k] == ninf ? 0.0f : ref[k];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float e = ex2(p[k][i] - base_ref);
+                for (int n = 0; n < 8; n++) {
+                    const float e = ex2(p[k][n] - base_ref);
                     sum[k] += e;
-                    p[k][i] = e * (i < 4 ? r0 : r1);
+                    p[k][n] = e * (n < 4 ? r0 : r1);
                 }
             }
-            // O += P V
+            uint32_t pa[2][4];
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
-                uint32_t pa[4];
                 if constexpr (SPLIT) {
                     const float *pp = &p[0][4 * ks];
                     const __half2 h0 = __floats2half2_rn(pp[0], pp[1]), h1 = __floats2half2_rn(pp[2], pp[3]);
-                    pa[0] = h2u(h0);
-                    pa[2] = h2u(h1);
-                    pa[1] = pack_h2(pp[0] - __low2float(h0), pp[1] - __high2float(h0));
-                    pa[3] = pack_h2(pp[2] - __low2float(h1), pp[3] - __high2float(h1));
+                    pa[ks][0] = h2u(h0);
+                    pa[ks][2] = h2u(h1);
+                    pa[ks][1] = pack_h2(pp[0] - __low2float(h0), pp[1] - __high2float(h0));
+                    pa[ks][3] = pack_h2(pp[2] - __low2float(h1), pp[3] - __high2float(h1));
                 } else {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
-                        pa[k] = pack_h2(p[k][4 * ks], p[k][4 * ks + 1]);
-                        pa[k + 2] = pack_h2(p[k][4 * ks + 2], p[k][4 * ks + 3]);
+                        pa[ks][k] = pack_h2(p[k][4 * ks], p[k][4 * ks + 1]);
+                        pa[ks][k + 2] = pack_h2(p[k][4 * ks + 2], p[k][4 * ks + 3]);
                     }
                 }
+            }
+            if (!mbar_wait_bounded(v_bar, uint32_t(vc) & 1u)) dead = true;
+            dead = __any_sync(0xffffffffu, dead);
+            if (dead) break;
+            // O += P V
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
                 // e4m3: bytes of keys that are not there may be NaN, which 0 * NaN would keep
                 uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
                 if constexpr (FMT != CPQ_KV_INT8) {
-                    const bool in = ks ? in1 : in0;
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        keep[i] = in && key0 + 16 * ks + 2 * tq + (i & 1) + 8 * (i >> 1) < u.seq.kv ? ~0u : 0u;
+                    for (int n = 0; n < 4; n++)
+                        keep[n] = (ks ? in1 : in0) && key0 + 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1) < u.seq.kv ? ~0u : 0u;
                 }
 #pragma unroll
                 for (int at = 0; at < NA; at++) {
                     uint4 vw[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int key = 16 * ks + 2 * tq + (i & 1) + 8 * (i >> 1);
-                        vw[i] = *reinterpret_cast<const uint4 *>(sv + at * (kAttnTile * 128) + key * 128 + ((gq ^ (key & 7)) << 4));
+                    for (int n = 0; n < 4; n++) {
+                        const int key = 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1);
+                        vw[n] = *reinterpret_cast<const uint4 *>(my_v + at * at_stride + ks * half_skip + key * 128 + ((gq ^ (key & 7)) << 4));
                     }
 #pragma unroll
                     for (int wi = 0; wi < 4; wi++) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            w[i] = wi == 0 ? vw[i].x : wi == 1 ? vw[i].y : wi == 2 ? vw[i].z : vw[i].w;
-                            if constexpr (FMT != CPQ_KV_INT8) w[i] &= keep[i];
+                        for (int n = 0; n < 4; n++) {
+                            w[n] = wi == 0 ? vw[n].x : wi == 1 ? vw[n].y : wi == 2 ? vw[n].z : vw[n].w;
+                            if constexpr (FMT != CPQ_KV_INT8) w[n] &= keep[n];
                         }
                         uint32_t b[4][2];
                         codes_h2<FMT>(__byte_perm(w[0], w[1], 0x5140), b[0][0], b[1][0]);
@@ -623,16 +637,19 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                         codes_h2<FMT>(__byte_perm(w[2], w[3], 0x5140), b[0][1], b[1][1]);
                         codes_h2<FMT>(__byte_perm(w[2], w[3], 0x7362), b[2][1], b[3][1]);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) mma_f16(o[at * 16 + wi * 4 + i], pa, b[i][0], b[i][1]);
+                        for (int n = 0; n < 4; n++) mma_f16(o[at * 16 + wi * 4 + n], pa[ks], b[n][0], b[n][1]);
                     }
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[st]);
+            if (i + 1 < n_own) copy((i + 1) / 32 == i / 32 ? cur : nxt, i + 1, &a.tmap_v, my_v, v_bar);
         }
-        base += n_here;
 
-        // join the eight warps: stats first, then the accumulators at the common reference
+        // join the warps: stats first, then the accumulators at the common reference. The next unit's first
+        // copies of K go out meanwhile.
+        const AttnUnit done = u;
+        more = walk.next(u);
+        if (more) begin();
 #pragma unroll
         for (int k = 0; k < NR; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
@@ -640,54 +657,55 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
             if (tq == 0) stat[warp * 16 + gq + 8 * k] = make_float2(ref[k], sum[k]);
         }
         if (lane == 0) vstat[warp] = vref;
-        dec_sync();
+        __syncthreads();
         float top[NR], all[NR];
 #pragma unroll
         for (int k = 0; k < NR; k++) {
             top[k] = ninf;
             all[k] = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; w++) top[k] = fmaxf(top[k], stat[w * 16 + gq + 8 * k].x);
+            for (int w = 0; w < W; w++) top[k] = fmaxf(top[k], stat[w * 16 + gq + 8 * k].x);
             const float b = top[k] == ninf ? 0.0f : top[k];
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; w++) {
+            for (int w = 0; w < W; w++) {
                 const float2 x = stat[w * 16 + gq + 8 * k];
                 all[k] += x.y * ex2(x.x - b);
             }
         }
         // fragment order: [16 at + b][row][n], dim 128 at + 16 n + b
         float *mine = red + (warp & 3) * (kRows * D);
-        auto put = [&](bool add) {
+#pragma unroll 1
+        for (int r = W / 4 - 1; r >= 0; r--) {  // four warps at a time
+            if ((warp >> 2) == r) {
 #pragma unroll
-            for (int k = 0; k < NR; k++) {
-                const float f = ex2(ref[k] - (top[k] == ninf ? 0.0f : top[k])) * vref;
+                for (int k = 0; k < NR; k++) {
+                    const float f = ex2(ref[k] - (top[k] == ninf ? 0.0f : top[k])) * vref;
 #pragma unroll
-                for (int i = 0; i < D / 8; i++) {
-                    float2 *to = reinterpret_cast<float2 *>(mine + (i * kRows + gq + 8 * k) * 8 + 2 * tq);
-                    float2 v = SPLIT ? make_float2((o[i][0] + o[i][2]) * f, (o[i][1] + o[i][3]) * f)
-                                     : make_float2(o[i][2 * k] * f, o[i][2 * k + 1] * f);
-                    if (add) {
-                        const float2 w = *to;
-                        v.x += w.x, v.y += w.y;
+                    for (int i = 0; i < D / 8; i++) {
+                        float2 *to = reinterpret_cast<float2 *>(mine + (i * kRows + gq + 8 * k) * 8 + 2 * tq);
+                        float2 v = SPLIT ? make_float2((o[i][0] + o[i][2]) * f, (o[i][1] + o[i][3]) * f)
+                                         : make_float2(o[i][2 * k] * f, o[i][2 * k + 1] * f);
+                        if (r != W / 4 - 1) {
+                            const float2 w = *to;
+                            v.x += w.x, v.y += w.y;
+                        }
+                        *to = v;
                     }
-                    *to = v;
                 }
             }
-        };
-        if (warp >= 4) put(false);
-        dec_sync();
-        if (warp < 4) put(true);
-        if (warp == 0 && tq == 0) {
-#pragma unroll
-            for (int k = 0; k < NR; k++) stat[gq + 8 * k] = make_float2(top[k], all[k]);
+            __syncthreads();
         }
-        dec_sync();
-        const bool whole = u.t0 == 0 && u.t1 == u.n;
-        const int slot = attn_slot(u);
-        for (int i = threadIdx.x; i < kRows * (D / 16); i += 32 * kAttnWarps) {
+        const bool whole = done.t0 == 0 && done.t1 == done.n;
+        const int slot = attn_slot(done);
+        for (int i = threadIdx.x; i < kRows * (D / 16); i += C::kThreads) {
             const int n = i & 7, rr = (i >> 3) % kRows, at = (i >> 3) / kRows;
-            const int row = u.r * kRows + rr;
-            const bool there = row < u.seq.q * a.group;
+            const int row = done.r * kRows + rr;
+            const bool there = row < done.seq.q * a.group;
+            float2 ml = make_float2(ninf, 0.0f);  // the row's statistics, as above
+#pragma unroll
+            for (int w = 0; w < W; w++) ml.x = fmaxf(ml.x, stat[w * 16 + rr].x);
+#pragma unroll
+            for (int w = 0; w < W; w++) ml.y += stat[w * 16 + rr].y * ex2(stat[w * 16 + rr].x - (ml.x == ninf ? 0.0f : ml.x));
             float v[16];
 #pragma unroll
             for (int b = 0; b < 16; b++) {
@@ -695,11 +713,10 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
                 v[b] = (red[e] + red[kRows * D + e]) + (red[2 * kRows * D + e] + red[3 * kRows * D + e]);
             }
             const int d0 = at * 128 + n * 16;
-            const float2 ml = stat[rr];
             if (whole) {
                 if (there) {
                     const float f = attn_inverse(ml.y);
-                    const int tok = u.seq.row0 + row / a.group, head = u.h * a.group + row % a.group;
+                    const int tok = done.seq.row0 + row / a.group, head = done.h * a.group + row % a.group;
                     const int64_t to = tok * a.os_tok + head * a.os_head + d0;
 #pragma unroll
                     for (int b = 0; b < 16; b++) attn_out_at(a, to + b, v[b] * f);
@@ -710,11 +727,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_decode_kernel(const __gr
 #pragma unroll
                 for (int b = 0; b < 4; b++) to[b] = make_float4(v[4 * b], v[4 * b + 1], v[4 * b + 2], v[4 * b + 3]);
                 if (d0 == 0) a.part_ml[slot * kRows + rr] = ml;
-                if (i == 0) a.part_hdr[slot] = make_int4(u.s, u.r, u.h, u.t1 == u.n ? 2 : 1);
+                if (i == 0) a.part_hdr[slot] = make_int4(done.s, done.r, done.h, done.t1 == done.n ? 2 : 1);
             }
         }
-        // q, stats and sums are rewritten by the next unit only after everyone is done with them
-        dec_sync();
+        gave_up = __syncthreads_or(dead) != 0;  // one warp's for all; q, stats and V's place are free again
+        fence_proxy_async_smem();               // the accumulators before the copies into their place
+    }
+    // no copy may land after the CTA has left: one that gave up may have some under way
+    if (gave_up) {
+        for (int i = 0; i < 2; i++) mbar_wait_bounded(&k_bar[i], uint32_t((kc + i) >> 1) & 1u);
+        mbar_wait_bounded(v_bar, uint32_t(vc) & 1u);
     }
 }
 

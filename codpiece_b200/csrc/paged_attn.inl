@@ -2,15 +2,16 @@
 
 namespace cpq {
 
-// The cache's codes as a byte matrix of head rows, box 128 bytes x up to 32 keys, 128-byte swizzle.
+// The cache's codes as [D / 128][head rows][128] bytes, box 128 bytes x up to 32 keys x all of D, 128-byte swizzle.
 static cpq_status kv_tensor_map(const cpq_kv_cache *c, const void *codes, CUtensorMap *out) {
     EncodeTiledFn enc = encode_tiled();
     if (!enc) return fail(CPQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[2] = {cuuint64_t(c->head_dim), cuuint64_t(c->n_pages) * cuuint64_t(c->n_head_kv) * cuuint64_t(c->block)};
-    const cuuint64_t strides[1] = {cuuint64_t(c->head_dim)};
-    const cuuint32_t box[2] = {128, cuuint32_t(std::min(c->block, kAttnTile))};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, estr,
+    const cuuint64_t rows = cuuint64_t(c->n_pages) * cuuint64_t(c->n_head_kv) * cuuint64_t(c->block);
+    const cuuint64_t dims[3] = {128, rows, cuuint64_t(c->head_dim / 128)};
+    const cuuint64_t strides[2] = {cuuint64_t(c->head_dim), 128};
+    const cuuint32_t box[3] = {128, cuuint32_t(std::min(c->block, kAttnTile)), cuuint32_t(c->head_dim / 128)};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(codes), dims, strides, box, estr,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? CPQ_SUCCESS : fail(CPQ_ERR_CUDA, "cuTensorMapEncodeTiled (kv cache) failed (%d)", int(r));
@@ -43,7 +44,7 @@ static cudaError_t launch_attn_decode(const AttnArgs &a, int ctas, cudaStream_t 
     using C = DecCfg<D, SPLIT>;
     cudaError_t e = raise_shared_limit<attn_decode_kernel<D, FMT, SPLIT>>(C::kSmem);
     if (e != cudaSuccess) return e;
-    e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(kAttnThreads), C::kSmem, st, a);
+    e = launch(attn_decode_kernel<D, FMT, SPLIT>, dim3(unsigned(ctas)), dim3(C::kThreads), C::kSmem, st, a);
     if (e != cudaSuccess) return e;
     return launch_attn_combine<D, C::kRows>(a, ctas, st);
 }
@@ -150,7 +151,7 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     a.causal = causal ? 1 : 0;
     a.scale_log2 = float(double(scale) * 1.4426950408889634);
     a.wide = wide_rows(q, 16) && wide_rows(out, 16) ? 1 : 0;
-    a.min_tiles = tc ? 4 : kAttnWarps;
+    a.min_share = tc ? 6 : 16;
     attn_carve(a, workspace, ctas, unit_rows, c->head_dim);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
     cudaError_t e;

@@ -61,6 +61,7 @@ constexpr int kTaQuarter = 32;    // keys of a V stage
 constexpr int kTaThreads = 896;
 constexpr int kTaConvWarps = 16;
 constexpr int kTaSoftWarps = 8;
+constexpr int kTaStart = 2;       // beginning a unit takes about as long as this many tiles
 constexpr int kTaInfo = 4;        // key tiles looked up ahead
 static_assert(kTaInfo == 4, "warp 1 looks up four tiles at a time");
 
@@ -325,16 +326,15 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
     pdl_wait();
     pdl_launch_dependents();
     tc_fence_before();
-    attn_make_plan<kTaRows, kTaTile>(a, plan, reinterpret_cast<int *>(sK));  // (its barriers also publish the TMEM address)
+    attn_make_plan<kTaRows, kTaTile, kTaStart>(a, plan, reinterpret_cast<int *>(sK));  // (its barriers also publish the TMEM address)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     // g: key tiles of this CTA so far, over units; parities and the info slot follow from it
-    const int n_tiles = plan.left;
 
     if (warp < 4) {
         if (warp == 0 && elect_one()) {
             // ---- MMA issue ----
-            AttnWalk<kTaRows, kTaTile> walk(a, plan);
+            AttnWalk<kTaRows, kTaTile, kTaStart> walk(a, plan);
             AttnUnit u;
             constexpr uint32_t idesc_s = tc_idesc_f16(kTaRows, kTaTile);
             constexpr uint32_t idesc_o = tc_idesc_f16(kTaRows, D) | (1u << 16);  // B is MN-major
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             }
         } else if (warp == 1) {
             // ---- cache rows and scales of the key tiles: lane = (tile of four, 16 keys of eight) ----
-            AttnWalk<kTaRows, kTaTile> walk(a, plan);
+            AttnWalk<kTaRows, kTaTile, kTaStart> walk(a, plan);
             AttnUnit u;
             const int lb = a.block == 16 ? 4 : a.block == 32 ? 5 : a.block == 64 ? 6 : 7;
             int g = 0;
@@ -451,6 +451,12 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
         const int blk = d0 >> 6, unit = (d0 & 63) >> 3, swap = blk & 1;
         const uint8_t *const codes = (is_v ? a.v : a.k) + (key_in & 15) * D + d0;
         uint8_t *const dst0 = (is_v ? sV + blk * C::kVBlock : sK) + key_in * 128;
+        int n_tiles = 0;
+        {
+            AttnWalk<kTaRows, kTaTile, kTaStart> walk(a, plan);
+            AttnUnit u;
+            while (walk.next(u)) n_tiles += u.t1 - u.t0;
+        }
         const int n_jobs = per_tile * n_tiles;
         auto load = [&](int j, uint4 (&x)[kLoads]) {
             if (j >= n_jobs) return true;
@@ -504,7 +510,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
         __syncwarp();
     } else {
         // ---- softmax: row = lane of tensor memory, 64 of the tile's keys per thread ----
-        AttnWalk<kTaRows, kTaTile> walk(a, plan);
+        AttnWalk<kTaRows, kTaTile, kTaStart> walk(a, plan);
         AttnUnit u;
         const int hf = (warp - 4) >> 2;                     // which half of the keys, and of D
         const int rr = 32 * (warp & 3) + lane;
