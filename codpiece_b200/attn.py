@@ -19,6 +19,9 @@ device's current one. There is no CPU or PyTorch fallback.
 from __future__ import annotations
 
 import ctypes as C
+import struct
+import threading
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -34,21 +37,62 @@ _KV_TYPES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 _KV_DTYPES = {KV_INT8: torch.int8, KV_E4M3: torch.float8_e4m3fn}
 
 
-def _desc(t: torch.Tensor, what: str) -> CpqTensor:
-    """Descriptor of a [tokens, heads, D] activation tensor (ne = [D, heads, tokens, 1])."""
-    if not t.is_cuda or t.dtype not in _ACT_TYPES or t.dim() != 3:
+# The calls of this module stand between kernels of a few microseconds, so they are kept cheap: descriptors are
+# packed as bytes into a per-thread scratch (a thread's call has returned before its next one packs) and passed by
+# address, and the device is switched only when the tensors' is not the current one.
+_TENSOR = struct.Struct("i4x4q4QQ")      # cpq_tensor
+_CACHE = struct.Struct("4iq4Q")          # cpq_kv_cache
+_SEQS = struct.Struct("3Q2qi4x")         # cpq_attn_seqs
+_SLOT_ARGS = struct.Struct("2QqQq2iQqQ5Qq")  # cpq_kv_slot_args
+assert (_TENSOR.size, _CACHE.size, _SEQS.size, _SLOT_ARGS.size) == tuple(
+    C.sizeof(t) for t in (CpqTensor, CpqKvCache, CpqAttnSeqs, CpqKvSlotArgs))
+_SLOTS = 8  # tensor descriptors of a call at most
+
+
+class _Scratch(threading.local):
+    def __init__(self):
+        self.buf = C.create_string_buffer(_SLOTS * _TENSOR.size + 3 * 128 + _SLOTS * 8)
+        base = C.addressof(self.buf)
+        self.tensor = [base + i * _TENSOR.size for i in range(_SLOTS)]
+        self.at = _SLOTS * _TENSOR.size  # cache, sequences, slot arguments: 128 bytes each
+        self.cache, self.seqs, self.slots = (base + self.at + 128 * i for i in range(3))
+        # arrays of pointers to the descriptors: 0-3 inputs, 4-7 outputs
+        struct.pack_into(f"{_SLOTS}Q", self.buf, self.at + 384, *self.tensor)
+        self.inputs, self.outputs = base + self.at + 384, base + self.at + 384 + 32
+
+
+_scratch = _Scratch()
+_fast: C.CDLL | None = None
+
+
+def _calls() -> C.CDLL:
+    """The library with these entry points taking addresses as integers."""
+    global _fast
+    if _fast is None:
+        lib()
+        f = C.CDLL(str(_lib.LIB_PATH))
+        vp = C.c_void_p
+        for name, args in (("cpq_rope_apply", [vp, vp, vp, C.c_int, vp, vp]), ("cpq_kv_slots", [vp, vp]),
+                           ("cpq_kv_append", [vp] * 5), ("cpq_kv_gather", [vp] * 5),
+                           ("cpq_paged_attn", [vp, vp, vp, C.c_float, C.c_int32, vp, vp, vp, C.c_size_t, vp])):
+            getattr(f, name).argtypes, getattr(f, name).restype = args, C.c_int
+        f.cpq_paged_attn_workspace_size.argtypes, f.cpq_paged_attn_workspace_size.restype = [vp, vp, C.c_int64], C.c_size_t
+        _fast = f
+    return _fast
+
+
+def _put(sc: _Scratch, i: int, t: torch.Tensor, what: str) -> int:
+    """Packs descriptor i from a [tokens, heads, D] activation tensor (ne = [D, heads, tokens, 1]); its address."""
+    typ = _ACT_TYPES.get(t.dtype)
+    if typ is None or not t.is_cuda or t.dim() != 3:
         raise TypeError(f"{what}: expected a CUDA tensor [tokens, heads, D] of float32, float16 or bfloat16")
-    if t.stride(2) != 1 and t.shape[2] != 1:
-        raise TypeError(f"{what}: rows must be contiguous (stride {t.stride(2)} along the last dimension)")
-    if min(t.stride()) < 0:
-        raise TypeError(f"{what}: negative stride")
-    b = t.element_size()
-    d = CpqTensor()
-    d.type = _ACT_TYPES[t.dtype]
-    d.ne[:] = [t.shape[2], t.shape[1], t.shape[0], 1]
-    d.nb[:] = [b, t.stride(1) * b, t.stride(0) * b, t.stride(0) * b * t.shape[0]]
-    d.data = t.data_ptr()
-    return d
+    n, h, d = t.shape
+    sn, sh, sd = t.stride()
+    if sd != 1 and d != 1:
+        raise TypeError(f"{what}: rows must be contiguous (stride {sd} along the last dimension)")
+    b = 4 if typ == _lib.TYPE_F32 else 2
+    _TENSOR.pack_into(sc.buf, i * _TENSOR.size, typ, d, h, n, 1, b, sh * b, sn * b, sn * b * n, t.data_ptr())
+    return sc.tensor[i]
 
 
 def _check_ints(t: torch.Tensor, what: str, dtype: torch.dtype, device: torch.device, numel: int | None = None) -> None:
@@ -66,20 +110,35 @@ def _table(table: torch.Tensor, n: int, device: torch.device) -> int:
     """Row stride of a block table [n, max_blocks]."""
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != n or table.device != device:
         raise TypeError(f"block table: expected an int32 tensor [{n}, blocks] on {device}")
-    if table.shape[1] > 1 and table.stride(1) != 1:
+    blocks = table.shape[1]
+    row, col = table.stride()
+    if blocks > 1 and col != 1:
         raise TypeError("block table: rows must be contiguous")
-    stride = table.stride(0) if n > 1 else table.shape[1]
-    if stride < table.shape[1]:
+    stride = row if n > 1 else blocks
+    if stride < blocks:
         raise TypeError("block table: rows overlap")
     return stride
 
 
-def _stream(stream, device: torch.device) -> C.c_void_p:
-    return C.c_void_p((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+_same = nullcontext()
 
 
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else C.c_void_p(t.data_ptr())
+def _on(device: torch.device):
+    """The device's context, when it is not the current one."""
+    return _same if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(stream, device: torch.device) -> int:
+    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+
+
+def _allocating(stream):
+    """Tensors made under this belong to the call's stream."""
+    return _same if stream is None else torch.cuda.stream(stream)
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 # ---- rotary positions ----------------------------------------------------------------
@@ -112,22 +171,24 @@ def rope(table: Rope, xs: list[torch.Tensor], pos: torch.Tensor, outs: list[torc
          stream=None) -> list[torch.Tensor]:
     """xs (q and k, up to 4 tensors [T, heads, D] of one type) rotated to pos [T] (int32).
     outs may be xs itself: rotated in place."""
-    if not 1 <= len(xs) <= 4:
-        raise ValueError(f"{len(xs)} tensors (1 to 4)")
+    n = len(xs)
+    if not 1 <= n <= 4:
+        raise ValueError(f"{n} tensors (1 to 4)")
     dev = xs[0].device
     if outs is None:
-        outs = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
-    if len(outs) != len(xs):
-        raise ValueError(f"{len(outs)} outputs for {len(xs)} tensors")
+        with _allocating(stream):
+            outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs]
+    if len(outs) != n:
+        raise ValueError(f"{len(outs)} outputs for {n} tensors")
     _check_ints(pos, "pos", torch.int32, dev, xs[0].shape[0])
-    for t in [*xs, *outs]:
-        _same_device(dev, tensor=t)
-    n = len(xs)
-    xd, yd = [_desc(t, "rope") for t in xs], [_desc(t, "rope out") for t in outs]
-    xa = (C.POINTER(CpqTensor) * n)(*[C.pointer(d) for d in xd])
-    ya = (C.POINTER(CpqTensor) * n)(*[C.pointer(d) for d in yd])
-    with torch.cuda.device(dev):
-        check(lib().cpq_rope_apply(table.handle, xa, ya, n, _ptr(pos), _stream(stream, dev)), "cpq_rope_apply")
+    sc = _scratch
+    for i in range(n):
+        _put(sc, i, xs[i], "rope")
+        _put(sc, 4 + i, outs[i], "rope out")
+        if xs[i].device != dev or outs[i].device != dev:
+            raise ValueError(f"rope: tensors on {dev} and another device")
+    with _on(dev):
+        check(_calls().cpq_rope_apply(table.handle, sc.inputs, sc.outputs, n, pos.data_ptr(), _stream(stream, dev)), "cpq_rope_apply")
     return outs
 
 
@@ -188,9 +249,11 @@ class KvCache:
     def device(self) -> torch.device:
         return self.k.device
 
-    def desc(self) -> CpqKvCache:
-        return CpqKvCache(_KV_TYPES[self.k.dtype], self.head_dim, self.n_head_kv, self.block, self.n_pages,
-                          self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr())
+    def _put(self, sc: _Scratch) -> int:
+        p, h, b, d = self.k.shape
+        _CACHE.pack_into(sc.buf, sc.at, _KV_TYPES[self.k.dtype], d, h, b, p, self.k.data_ptr(), self.v.data_ptr(),
+                         self.k_scale.data_ptr(), self.v_scale.data_ptr())
+        return sc.cache
 
 
 @dataclass
@@ -211,22 +274,26 @@ def kv_slots(ctx_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor, 
     dev, n = ctx_len.device, ctx_len.numel()
     taken_out = taken if taken_out is None else taken_out
     if out is None:
-        ints = lambda m, dt=torch.int32: torch.empty(m, dtype=dt, device=dev)  # noqa: E731
-        out = Slots(ints(n + 1), ints(n), ints(n_rows), ints(n_rows, torch.int64))
-    for name, t, dt, m in (("ctx_len", ctx_len, torch.int32, n), ("new_len", new_len, torch.int32, n),
-                           ("free_pages", free_pages, torch.int32, None), ("taken", taken, torch.int32, 1),
-                           ("taken_out", taken_out, torch.int32, 1), ("seq_start", out.seq_start, torch.int32, n + 1),
-                           ("kv_len", out.kv_len, torch.int32, n), ("pos", out.pos, torch.int32, n_rows),
-                           ("slot", out.slot, torch.int64, n_rows)):
-        _check_ints(t, name, dt, dev, m)
+        with _allocating(stream):
+            out = Slots(torch.empty(n + 1, dtype=torch.int32, device=dev), torch.empty(n, dtype=torch.int32, device=dev),
+                        torch.empty(n_rows, dtype=torch.int32, device=dev), torch.empty(n_rows, dtype=torch.int64, device=dev))
+    else:
+        for name, t, dt, m in (("seq_start", out.seq_start, torch.int32, n + 1), ("kv_len", out.kv_len, torch.int32, n),
+                               ("pos", out.pos, torch.int32, n_rows), ("slot", out.slot, torch.int64, n_rows)):
+            _check_ints(t, name, dt, dev, m)
+    for name, t, m in (("ctx_len", ctx_len, n), ("new_len", new_len, n), ("free_pages", free_pages, None), ("taken", taken, 1),
+                       ("taken_out", taken_out, 1)):
+        _check_ints(t, name, torch.int32, dev, m)
     if not ctx_len.is_cuda:
         raise TypeError("kv_slots: expected CUDA tensors")
     stride = _table(table, n, dev)
-    a = CpqKvSlotArgs(ctx_len.data_ptr(), new_len.data_ptr(), n, table.data_ptr(), stride, table.shape[1], block,
-                      free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(), taken_out.data_ptr(),
-                      out.seq_start.data_ptr(), out.kv_len.data_ptr(), out.pos.data_ptr(), out.slot.data_ptr(), n_rows)
-    with torch.cuda.device(dev):
-        check(lib().cpq_kv_slots(C.byref(a), _stream(stream, dev)), "cpq_kv_slots")
+    sc = _scratch
+    _SLOT_ARGS.pack_into(sc.buf, sc.at + 256, ctx_len.data_ptr(), new_len.data_ptr(), n, table.data_ptr(), stride,
+                         table.shape[1], block, free_pages.data_ptr(), free_pages.numel(), taken.data_ptr(),
+                         taken_out.data_ptr(), out.seq_start.data_ptr(), out.kv_len.data_ptr(), out.pos.data_ptr(),
+                         out.slot.data_ptr(), n_rows)
+    with _on(dev):
+        check(_calls().cpq_kv_slots(sc.slots, _stream(stream, dev)), "cpq_kv_slots")
     return out
 
 
@@ -236,10 +303,10 @@ def kv_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slot: torch.Tens
     dev = cache.device
     _same_device(dev, k=k, v=v)
     _check_ints(slot, "slot", torch.int64, dev, k.shape[0])
-    cd, kd, vd = cache.desc(), _desc(k, "k"), _desc(v, "v")
-    with torch.cuda.device(dev):
-        check(lib().cpq_kv_append(C.byref(cd), C.byref(kd), C.byref(vd), _ptr(slot), _stream(stream, dev)),
-              "cpq_kv_append")
+    sc = _scratch
+    with _on(dev):
+        check(_calls().cpq_kv_append(cache._put(sc), _put(sc, 0, k, "k"), _put(sc, 1, v, "v"), slot.data_ptr(),
+                                     _stream(stream, dev)), "cpq_kv_append")
 
 
 def kv_gather(cache: KvCache, slot: torch.Tensor, dtype: torch.dtype = torch.float32,
@@ -247,17 +314,19 @@ def kv_gather(cache: KvCache, slot: torch.Tensor, dtype: torch.dtype = torch.flo
     """The values of slots [T] (int64) as k, v [T, n_head_kv, D]; rows outside the pool are zeros."""
     dev = cache.device
     _check_ints(slot, "slot", torch.int64, dev)
+    n = slot.numel()
     if outs is None:
-        shape = (slot.numel(), cache.n_head_kv, cache.head_dim)
-        outs = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+        shape = (n, cache.n_head_kv, cache.head_dim)
+        with _allocating(stream):
+            outs = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
     k, v = outs
     _same_device(dev, k=k, v=v)
-    if k.shape[0] != slot.numel():
-        raise ValueError(f"{k.shape[0]} rows for {slot.numel()} slots")
-    cd, kd, vd = cache.desc(), _desc(k, "k"), _desc(v, "v")
-    with torch.cuda.device(dev):
-        check(lib().cpq_kv_gather(C.byref(cd), _ptr(slot), C.byref(kd), C.byref(vd), _stream(stream, dev)),
-              "cpq_kv_gather")
+    if k.shape[0] != n:
+        raise ValueError(f"{k.shape[0]} rows for {n} slots")
+    sc = _scratch
+    with _on(dev):
+        check(_calls().cpq_kv_gather(cache._put(sc), slot.data_ptr(), _put(sc, 0, k, "k"), _put(sc, 1, v, "v"),
+                                     _stream(stream, dev)), "cpq_kv_gather")
     return k, v
 
 
@@ -279,27 +348,26 @@ def paged_attn(q: torch.Tensor, cache: KvCache, table: torch.Tensor, seq_start: 
     _check_ints(seq_start, "seq_start", torch.int32, dev, n + 1)
     _check_ints(kv_len, "kv_len", torch.int32, dev, n)
     stride = _table(table, n, dev)
-    qd, cd = _desc(q, "q"), cache.desc()
+    sc = _scratch
+    qd, cd = _put(sc, 0, q, "q"), cache._put(sc)
     if scale is None:
         scale = cache.head_dim ** -0.5
-    s = stream if stream is not None else torch.cuda.current_stream(dev)
-    with torch.cuda.device(dev), torch.cuda.stream(s):
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        if lse is None and return_lse:
-            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-        need = lib().cpq_paged_attn_workspace_size(C.byref(cd), C.byref(qd), n)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    _same_device(dev, out=out, lse=lse, workspace=workspace)
-    if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
-        raise TypeError(f"lse: expected a contiguous float32 tensor {tuple(q.shape[:2])}")
-    if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise TypeError("workspace: expected a contiguous uint8 tensor")
-    od = _desc(out, "out")
-    seqs = CpqAttnSeqs(seq_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(), stride, n, table.shape[1])
-    with torch.cuda.device(dev):
-        check(lib().cpq_paged_attn(C.byref(qd), C.byref(cd), C.byref(seqs), scale, 1 if causal else 0, C.byref(od),
-                                   _ptr(lse), _ptr(workspace), workspace.numel(), C.c_void_p(s.cuda_stream)),
-              "cpq_paged_attn")
+    calls = _calls()
+    with _on(dev):
+        with _allocating(stream):
+            if out is None:
+                out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            if lse is None and return_lse:
+                lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+            if workspace is None:
+                workspace = torch.empty(calls.cpq_paged_attn_workspace_size(cd, qd, n), dtype=torch.uint8, device=dev)
+        _same_device(dev, out=out, lse=lse, workspace=workspace)
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+            raise TypeError(f"lse: expected a contiguous float32 tensor {tuple(q.shape[:2])}")
+        if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+            raise TypeError("workspace: expected a contiguous uint8 tensor")
+        od = _put(sc, 1, out, "out")
+        _SEQS.pack_into(sc.buf, sc.at + 128, seq_start.data_ptr(), kv_len.data_ptr(), table.data_ptr(), stride, n, table.shape[1])
+        check(calls.cpq_paged_attn(qd, cd, sc.seqs, scale, 1 if causal else 0, od, _ptr(lse), workspace.data_ptr(),
+                                   workspace.numel(), _stream(stream, dev)), "cpq_paged_attn")
     return (out, lse) if return_lse else out

@@ -303,9 +303,10 @@ constexpr int kAttnTile = 32;
 
 template <int D, bool SPLIT> struct DecCfg {
     static constexpr int kRows = SPLIT ? 8 : 16;
-    static constexpr int kWarps = D == 256 ? 8 : 12;             // D = 256: 255 registers, D = 128: 168
+    static constexpr int kWarps = 8;                             // 255 registers (12 warps of 168: D = 128 spills, 10 % slower)
+    static constexpr bool kEarlyQ = D == 128;                    // room to hold the next unit's q while one ends
     static constexpr int kThreads = 32 * kWarps;
-    static constexpr int kStart = kWarps;                        // beginning a unit takes about as long as a tile per warp
+    static constexpr int kStart = 32;                            // beginning a unit takes about as long as this many tiles (4 to 32 tried)
     static constexpr int kCodes = kAttnTile * D;                 // K or V codes of a tile
     static constexpr int kVOff = kWarps * 2 * kCodes;            // K: two slots per warp; V: one
     static constexpr int kQOff = kVOff + kWarps * kCodes;
@@ -424,24 +425,38 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
         if (n_own > 0) copy(cur, 0, &a.tmap_k, my_k + (kc & 1) * C::kCodes, &k_bar[kc & 1]);
         if (n_own > 1) copy(cur, 1, &a.tmap_k, my_k + ((kc + 1) & 1) * C::kCodes, &k_bar[(kc + 1) & 1]);
     };
+    // the unit's q rows of this warp, E elements per lane, in flight while the unit before ends
+    constexpr int E = D / 32, QR = (kRows + W - 1) / W;
+    float qx[QR][E];
+    auto load_q = [&]() {
+#pragma unroll
+        for (int k = 0; k < QR; k++) {
+            const int rr = warp + W * k, row = u.r * kRows + rr;
+            const bool there = rr < kRows && row < u.seq.q * a.group;
+            const int tok = u.seq.row0 + row / a.group, head = u.h * a.group + row % a.group;
+            const int64_t at = tok * a.qs_tok + head * a.qs_head + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; e++) qx[k][e] = there ? attn_q_at(a, at + e) : 0.0f;
+        }
+    };
     const int gq = lane >> 2, tq = lane & 3;
     bool more = walk.next(u);
-    if (more) begin();
+    if (more) {
+        if (C::kEarlyQ) load_q();
+        begin();
+    }
     bool gave_up = false;
     while (more && !gave_up) {
         if (n_own > 0) copy(cur, 0, &a.tmap_v, my_v, v_bar);
         // q of the unit's rows, as A fragments in the K order above
-        for (int rr = warp; rr < kRows; rr += W) {
-            const int row = u.r * kRows + rr;
-            const bool there = row < u.seq.q * a.group;
-            constexpr int E = D / 32;
-            float x[E], m = 0.0f;
-            const int tok = u.seq.row0 + row / a.group, head = u.h * a.group + row % a.group;
+        if (!C::kEarlyQ) load_q();
 #pragma unroll
-            for (int e = 0; e < E; e++) {
-                x[e] = there ? attn_q_at(a, tok * a.qs_tok + head * a.qs_head + lane * E + e) : 0.0f;
-                m = fmaxf(m, fabsf(x[e]));
-            }
+        for (int k = 0; k < QR; k++) {
+            const int rr = warp + W * k;
+            if (rr >= kRows) break;
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; e++) m = fmaxf(m, fabsf(qx[k][e]));
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             const int sh = attn_q_shift(m);
@@ -453,9 +468,9 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
                 uint32_t *to = reinterpret_cast<uint32_t *>(sq + ((d >> 7) * 8 + ((d >> 2) & 7)) * 32 + (rr & 7) * 4 + ((d >> 5) & 3));
                 float hi[4], lo[4];
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    hi[k] = __half2float(__float2half_rn(x[e + k] * f));
-                    lo[k] = x[e + k] * f - hi[k];
+                for (int i = 0; i < 4; i++) {
+                    hi[i] = __half2float(__float2half_rn(qx[k][e + i] * f));
+                    lo[i] = qx[k][e + i] * f - hi[i];
                 }
                 to[rr >> 3] = pack_h2(hi[0], hi[1]);
                 to[2 + (rr >> 3)] = pack_h2(hi[2], hi[3]);
@@ -649,7 +664,10 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
         // copies of K go out meanwhile.
         const AttnUnit done = u;
         more = walk.next(u);
-        if (more) begin();
+        if (more) {
+            if (C::kEarlyQ) load_q();
+            begin();
+        }
 #pragma unroll
         for (int k = 0; k < NR; k++) {
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);

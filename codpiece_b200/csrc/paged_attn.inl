@@ -151,7 +151,7 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     a.causal = causal ? 1 : 0;
     a.scale_log2 = float(double(scale) * 1.4426950408889634);
     a.wide = wide_rows(q, 16) && wide_rows(out, 16) ? 1 : 0;
-    a.min_share = tc ? 6 : 16;
+    a.min_share = tc ? 1 : 4;  // short requests are spread wide: latency counts, joining costs little
     attn_carve(a, workspace, ctas, unit_rows, c->head_dim);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
     cudaError_t e;
