@@ -128,8 +128,14 @@ def _on(device: torch.device):
     return _same if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+# the device's current stream without the Stream object around it (2 us a call), where torch has the call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(stream, device: torch.device) -> int:
-    return (stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 def _allocating(stream):
@@ -162,7 +168,7 @@ class Rope:
         check(lib().cpq_rope_create(C.byref(p), C.byref(self.handle)), "cpq_rope_create")
 
     def __del__(self):
-        if getattr(self, "handle", None):
+        if getattr(self, "handle", None) and lib is not None:  # (None while the interpreter shuts down)
             lib().cpq_rope_destroy(self.handle)
             self.handle = C.c_void_p()
 
@@ -177,7 +183,7 @@ def rope(table: Rope, xs: list[torch.Tensor], pos: torch.Tensor, outs: list[torc
     dev = xs[0].device
     if outs is None:
         with _allocating(stream):
-            outs = [torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs]
+            outs = [torch.empty_like(x) for x in xs]
     if len(outs) != n:
         raise ValueError(f"{len(outs)} outputs for {n} tensors")
     _check_ints(pos, "pos", torch.int32, dev, xs[0].shape[0])
@@ -316,9 +322,9 @@ def kv_gather(cache: KvCache, slot: torch.Tensor, dtype: torch.dtype = torch.flo
     _check_ints(slot, "slot", torch.int64, dev)
     n = slot.numel()
     if outs is None:
-        shape = (n, cache.n_head_kv, cache.head_dim)
+        _, h, _, d = cache.k.shape
         with _allocating(stream):
-            outs = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+            outs = (torch.empty(n, h, d, dtype=dtype, device=dev), torch.empty(n, h, d, dtype=dtype, device=dev))
     k, v = outs
     _same_device(dev, k=k, v=v)
     if k.shape[0] != n:
@@ -356,9 +362,9 @@ def paged_attn(q: torch.Tensor, cache: KvCache, table: torch.Tensor, seq_start: 
     with _on(dev):
         with _allocating(stream):
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+                out = torch.empty_like(q)
             if lse is None and return_lse:
-                lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+                lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=dev)
             if workspace is None:
                 workspace = torch.empty(calls.cpq_paged_attn_workspace_size(cd, qd, n), dtype=torch.uint8, device=dev)
         _same_device(dev, out=out, lse=lse, workspace=workspace)
