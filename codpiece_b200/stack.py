@@ -4,11 +4,13 @@ This is the benchmark's multi-GPU workload: n_layer layers of random-init
 Q4_K projections (hidden 5120, q 6144, k/v 1024, FFN 17408) and a Q6_K LM
 head over vocab 151936, run as decode (M = 1) or verify (M = 2..16) steps.
 Each layer follows codpiece's qwen35 trunk (crates/codpiece-model/src/
-qwen35.rs:2554-2786) with the attention core left out:
+qwen35.rs:2554-2786); the attention core is left out by default (the benchmark's
+stack) and runs when the stack is given an :class:`AttnCore`:
 
     xn = rms_norm(h)                             (2534-2537)
     q, k, v = W_q xn, W_k xn, W_v xn             (3029, 3047, 3051)
     h = h + allreduce(W_o q)                     (3197; q stands in for the attention output)
+      or, with an AttnCore: q, k rotated (3060-3120), k, v into the cache, W_o attention(q)
     xn = rms_norm(h)
     g, u = W_gate xn, W_up xn                    (2779-2780)
     h = h + allreduce(W_down (silu(g) * u))      (2781-2783)
@@ -28,6 +30,7 @@ from dataclasses import dataclass
 
 import torch
 
+from . import attn
 from . import mul_mat as mm
 from . import tp
 from ._lib import check, lib
@@ -79,12 +82,36 @@ class Comm:
             self.handle = C.c_void_p()
 
 
+class AttnCore:
+    """The attention core of a one-GPU stack's layers for one sequence: rotary frequencies, one paged
+    8-bit cache per layer, and the block table, page list and length they share (all on the device, so
+    a step can be captured and replayed; the length advances by the stack's M tokens per step). A step that
+    would pass max_ctx (rounded up to whole blocks) caches nothing, its attention gives zeros, the length stays."""
+
+    def __init__(self, hp: tp.Hparams, n_layer: int, max_ctx: int, block: int = 64, fmt: int = attn.KV_INT8,
+                 rope: attn.Rope | None = None, device="cuda"):
+        dev = torch.device(device)
+        pages = -(-max_ctx // block)
+        self.block = block
+        self.rope = rope if rope is not None else attn.Rope(hp.head_k // 4, attn.ROPE_HALF, base=1e7)
+        self.caches = [attn.KvCache.empty(pages, hp.n_head_kv, hp.head_k, block, fmt, device=dev) for _ in range(n_layer)]
+        i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        self.table = torch.full((1, pages), -1, dtype=torch.int32, device=dev)
+        self.free = torch.arange(pages, dtype=torch.int32, device=dev)
+        self.taken, self.ctx = i32(0), i32(0)
+
+    def rollback(self, n: int | torch.Tensor) -> None:
+        """Forgets the last n tokens (rejected by a verify step): their pages go back to the list."""
+        self.ctx.sub_(n).clamp_(min=0)
+        self.taken.copy_((self.ctx + (self.block - 1)) // self.block)
+
+
 class Stack:
     """This rank's shard of the stack plus its activation buffers."""
 
     def __init__(self, hp: tp.Hparams, n_layer: int, rank: int = 0, world: int = 1, comm: Comm | None = None,
                  m: int = 1, seed: int = 0, head: bool = True, device: int | None = None, eps: float = 1e-6,
-                 use_plan: bool = False, ar_exchange=None, use_trunk: bool = False):
+                 use_plan: bool = False, ar_exchange=None, use_trunk: bool = False, attn_core: AttnCore | None = None):
         self.hp, self.n_layer, self.rank, self.world, self.comm, self.m = hp, n_layer, rank, world, comm, m
         self.eps = eps
         self.dev = torch.device("cuda", torch.cuda.current_device() if device is None else device)
@@ -130,6 +157,16 @@ class Stack:
         self.h, self.h_alt, self.xn = f(e), f(e), f(e)
         self.h_final = self.h
         self.qb, self.kb, self.vb = f(qmax), f(kmax), f(kmax)
+        self.attn = attn_core
+        if attn_core is not None:
+            if world != 1 or use_plan or use_trunk:
+                raise ValueError("the attention core runs on one GPU, with per-call layers")
+            if len(attn_core.caches) != n_layer:
+                raise ValueError(f"{len(attn_core.caches)} caches for {n_layer} layers")
+            self.ab = f(qmax)
+            ints = lambda n, dt=torch.int32: torch.zeros(n, dtype=dt, device=self.dev)  # noqa: E731
+            self.new_len = torch.full((1,), m, dtype=torch.int32, device=self.dev)
+            self.slots = attn.Slots(ints(2), ints(1), ints(m), ints(m, torch.int64))
         self.part = f(e)
         self.gb, self.ub, self.act = f(fmax), f(fmax), f(fmax)
         self.logits = f(n_head) if head else None
@@ -180,6 +217,8 @@ class Stack:
             return 1 + (fused(mm.TYPE_Q6_K, True) + 1 if self.head is not None else 0)
         if self.plan is not None:
             return 1 + fused(mm.TYPE_Q6_K, True) + 1 if self.head is not None else 1
+        if self.attn is not None:
+            n += 1 + 4 * len(self.layers)  # slots; rope, append, attention and its join per layer
         for il, lw in enumerate(self.layers):
             if lw.q is not None or lw.k is not None or lw.v is not None:
                 n += fused(mm.TYPE_Q4_K, True)
@@ -248,6 +287,10 @@ class Stack:
         On return self.h holds the final residual stream."""
         h, h_alt = self.h, self.h_alt
         part_live = False  # self.part holds a projection output still to be added to h
+        core = self.attn
+        if core is not None:
+            attn.kv_slots(core.ctx, self.new_len, core.table, core.free, core.taken, block=core.block, n_rows=self.m,
+                          out=self.slots)
         if self.trunk is not None:
             self.trunk.run(h, h_alt)
             if self.head is not None:
@@ -260,7 +303,7 @@ class Stack:
             h, h_alt = self._plan_h
             part_live = len(self.layers) > 0
         ch = self.ar
-        for lw in ([] if self.plan is not None else self.layers):
+        for il, lw in enumerate([] if self.plan is not None else self.layers):
             # attention block: xn = rms(h [+ part]) -> q, k, v
             ws, outs = [], []
             for w, b in ((lw.q, self.qb), (lw.k, self.kb), (lw.v, self.vb)):
@@ -280,13 +323,17 @@ class Stack:
                     mm.add_(h, self.part)  # no attention rows on this rank: fold the residual in place
             elif ws:
                 mm.mul_mat_fused(ws, h, outs, mode=mm.PRO_RMS, eps=self.eps)
+            o_in = self.qb
+            if core is not None:
+                self._attention(il)
+                o_in = self.ab
             # o projection (row-parallel)
             if ch is not None and lw.o is not None:
                 mm.mul_mat_fused([lw.o], self._sl(self.qb, lw.o.k), [self.part], y_ar=ch)
             elif ch is not None:
                 ch.zero(self.hp.n_embd, self.m)  # no attention rows: a zero share of the all-reduce
             elif lw.o is not None:
-                mm.mul_mat(lw.o, self._sl(self.qb, lw.o.k), out=self.part)
+                mm.mul_mat(lw.o, self._sl(o_in, lw.o.k), out=self.part)
             else:
                 self.part.zero_()
             if self.world > 1 and ch is None:
@@ -322,7 +369,18 @@ class Stack:
             self._argmax()
         elif part_live:
             mm.add_(h, self.part)
+        if core is not None:
+            torch.maximum(core.ctx, self.slots.kv_len, out=core.ctx)  # a step that found no room leaves it
         self.h_final = h
+
+    def _attention(self, il: int) -> None:
+        """self.ab = the attention of self.qb over layer il's cache, with this step's k and v appended."""
+        core, cache = self.attn, self.attn.caches[il]
+        heads = lambda b, n: b.view(-1)[: self.m * n * cache.head_dim].view(self.m, n, cache.head_dim)  # noqa: E731
+        q, k, v = heads(self.qb, self.hp.n_head), heads(self.kb, self.hp.n_head_kv), heads(self.vb, self.hp.n_head_kv)
+        attn.rope(core.rope, [q, k], self.slots.pos, [q, k])
+        attn.kv_append(cache, k, v, self.slots.slot)
+        attn.paged_attn(q, cache, core.table, self.slots.seq_start, self.slots.kv_len, out=heads(self.ab, self.hp.n_head))
 
     def capture(self) -> None:
         """Capture step_body() into a CUDA graph (run one eager step first to warm up)."""
