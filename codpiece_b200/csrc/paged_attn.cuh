@@ -18,6 +18,14 @@
 // life (with 8 and 11 some row of a warp moved in every second or third tile,
 // and each time O is rescaled); a page's v_scale enters as its ratio to a
 // reference scale, which moves when a ratio exceeds 8. Sums are fp32.
+// The tensor cores cut a sum's bits below fp32 off instead of rounding them, so
+// every accumulation step loses a little on the same side (fp32 q, a row over
+// 9000 keys, 1130 steps: 1.6e-5 off in the 2-norm; 272 steps: 3.5e-6). After
+// some 100 steps the accumulators are therefore added into the workspace,
+// rounded to nearest (attn_flush4), and begin at 0 again, and second terms of q
+// and P are added before first ones, into small sums: 2.6e-6 and 1.9e-6 where
+// fp32 products and a fp32 softmax are 2.2e-6 off. The flushes cost 2 % of a decode
+// step over 100k keys, 7 % of a fp32 chunk (every 8 tiles instead of 6: 3 % less, 3.0e-6).
 //
 // Work. The query rows of one kv head and sequence, (token, head of the group)
 // in that order, form row tiles of kRows rows; a unit is (sequence, row tile,
@@ -63,7 +71,9 @@ struct alignas(64) AttnArgs {
     float *part_o;               // [slot][kRows][D]
     float2 *part_ml;             // [slot][kRows]: softmax reference, row sum
     int4 *part_hdr;              // [slot]: sequence, row tile, kv head, 0 unused | 1 goes on | 2 the unit's end
+    float4 *acc;                 // [CTA][kAttnAcc / 16 * D]: what accumulators held before; each element is one thread's
 };
+constexpr int kAttnAcc = 512;    // bytes of acc per CTA and dim (128 rows, or 8 warps of 16 accumulator rows)
 
 // ---- the split ------------------------------------------------------------------
 
@@ -259,6 +269,18 @@ __device__ __forceinline__ int attn_q_shift(float amax) {
 }
 __device__ __forceinline__ float attn_exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
+// Adds four accumulators to the workspace, or puts them there (a unit's first time). The additions of one thread to
+// one address come in its order: results repeat.
+__device__ __forceinline__ void attn_flush4(float4 *to, bool first, float a, float b, float c, float d) {
+    if (first) __stcg(to, make_float4(a, b, c, d));
+    else asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
+}
+// Scales what is there; reads it.
+__device__ __forceinline__ void attn_scale4(float4 *at, float f, float g) {
+    const float4 v = __ldcg(at);
+    __stcg(at, make_float4(v.x * f, v.y * f, v.z * g, v.w * g));
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -306,6 +328,8 @@ template <int D, bool SPLIT> struct DecCfg {
     static constexpr int kWarps = 8;                             // 255 registers (12 warps of 168: D = 128 spills, 10 % slower)
     static constexpr bool kEarlyQ = D == 128;                    // room to hold the next unit's q while one ends
     static constexpr int kThreads = 32 * kWarps;
+    // tiles (two accumulation steps each) between flushes; 16-bit outputs need none (what fits the memory: 2.6e-4 off)
+    static constexpr int kFlush = 64;
     static constexpr int kStart = 32;                            // beginning a unit takes about as long as this many tiles (4 to 32 tried)
     static constexpr int kCodes = kAttnTile * D;                 // K or V codes of a tile
     static constexpr int kVOff = kWarps * 2 * kCodes;            // K: two slots per warp; V: one
@@ -445,6 +469,12 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
         if (C::kEarlyQ) load_q();
         begin();
     }
+    auto flushed = [&]() {  // this lane's place for them (from special registers: none held meanwhile)
+        uint32_t cta, thread;
+        asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+        asm volatile("mov.u32 %0, %%tid.x;" : "=r"(thread));
+        return a.acc + (int64_t(cta) * W + (thread >> 5)) * (D / 8 * 32) + (thread & 31);
+    };
     bool gave_up = false;
     while (more && !gave_up) {
         if (n_own > 0) copy(cur, 0, &a.tmap_v, my_v, v_bar);
@@ -498,168 +528,193 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
             lim[k] = a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + row / a.group + 1) : u.seq.kv;
         }
         float vref = 0.0f;
-        for (int i = 0; i < n_own; i++, kc++, vc++) {
-            if ((i & 31) == 0) {  // lanes look at the warp's next 32 tiles, long before they are needed
-                cur = nxt;
-                if (i + 32 < n_own) nxt = look(i / 32 + 1);
-            }
-            const int key0 = (t_first + W * i) * kAttnTile;
-            const bool in0 = __shfl_sync(0xffffffffu, cur.page[0], i & 31) >= 0, in1 = __shfl_sync(0xffffffffu, cur.page[1], i & 31) >= 0;
-            const float ks0 = __shfl_sync(0xffffffffu, cur.ks[0], i & 31), ks1 = __shfl_sync(0xffffffffu, cur.ks[1], i & 31);
-            const float vs0 = __shfl_sync(0xffffffffu, cur.vs[0], i & 31), vs1 = __shfl_sync(0xffffffffu, cur.vs[1], i & 31);
-            const int st = kc & 1;
-            if (!dead && !mbar_wait_bounded(&k_bar[st], uint32_t(kc >> 1) & 1u)) dead = true;
-            dead = __any_sync(0xffffffffu, dead);
-            if (dead) break;
-            const uint8_t *const sk = my_k + st * C::kCodes;
-            float s[4][4];
+        for (int i = 0;;) {
+            const int stop = SPLIT ? min(n_own, i + C::kFlush) : n_own;
+            for (; i < stop; i++, kc++, vc++) {
+                if ((i & 31) == 0) {  // lanes look at the warp's next 32 tiles, long before they are needed
+                    cur = nxt;
+                    if (i + 32 < n_own) nxt = look(i / 32 + 1);
+                }
+                const int key0 = (t_first + W * i) * kAttnTile;
+                const bool in0 = __shfl_sync(0xffffffffu, cur.page[0], i & 31) >= 0, in1 = __shfl_sync(0xffffffffu, cur.page[1], i & 31) >= 0;
+                const float ks0 = __shfl_sync(0xffffffffu, cur.ks[0], i & 31), ks1 = __shfl_sync(0xffffffffu, cur.ks[1], i & 31);
+                const float vs0 = __shfl_sync(0xffffffffu, cur.vs[0], i & 31), vs1 = __shfl_sync(0xffffffffu, cur.vs[1], i & 31);
+                const int st = kc & 1;
+                if (!dead && !mbar_wait_bounded(&k_bar[st], uint32_t(kc >> 1) & 1u)) dead = true;
+                dead = __any_sync(0xffffffffu, dead);
+                if (dead) break;
+                const uint8_t *const sk = my_k + st * C::kCodes;
+                float s[4][4];
 #pragma unroll
-            for (int nt = 0; nt < 4; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+                for (int nt = 0; nt < 4; nt++) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
 #pragma unroll 1
-            for (int at = 0; at < NA; at++) {
-                uint4 kw[4][2];
+                for (int at = 0; at < NA; at++) {
+                    uint4 kw[4][2];
 #pragma unroll
-                for (int nt = 0; nt < 4; nt++)
+                    for (int nt = 0; nt < 4; nt++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
-                        kw[nt][c] = *reinterpret_cast<const uint4 *>(sk + at * at_stride + (nt >> 1) * half_skip + (8 * nt + gq) * 128 +
-                                                                     (((2 * tq + c) ^ gq) << 4));
+                        for (int c = 0; c < 2; c++)
+                            kw[nt][c] = *reinterpret_cast<const uint4 *>(sk + at * at_stride + (nt >> 1) * half_skip + (8 * nt + gq) * 128 +
+                                                                         (((2 * tq + c) ^ gq) << 4));
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint4 qw = sq[(at * 8 + j) * 32 + lane];
-                    const uint32_t qa[4] = {qw.x, qw.y, qw.z, qw.w};
+                    for (int j = 0; j < 8; j++) {
+                        const uint4 qw = sq[(at * 8 + j) * 32 + lane];
+                        const uint32_t qa[4] = {qw.x, qw.y, qw.z, qw.w};
 #pragma unroll
-                    for (int nt = 0; nt < 4; nt++) {
-                        const uint4 w = kw[nt][j >> 2];
-                        const uint32_t word = (j & 3) == 0 ? w.x : (j & 3) == 1 ? w.y : (j & 3) == 2 ? w.z : w.w;
-                        uint32_t b0, b1;
-                        codes_h2<FMT>(word, b0, b1);
-                        mma_f16(s[nt], qa, b0, b1);
+                        for (int nt = 0; nt < 4; nt++) {
+                            const uint4 w = kw[nt][j >> 2];
+                            const uint32_t word = (j & 3) == 0 ? w.x : (j & 3) == 1 ? w.y : (j & 3) == 2 ? w.z : w.w;
+                            uint32_t b0, b1;
+                            codes_h2<FMT>(word, b0, b1);
+                            mma_f16(s[nt], qa, b0, b1);
+                        }
                     }
                 }
-            }
-            __syncwarp();
-            if (i + 2 < n_own) copy((i + 2) / 32 == i / 32 ? cur : nxt, i + 2, &a.tmap_k, my_k + st * C::kCodes, &k_bar[st]);
-            // scores in log2, masked
-            float p[NR][8];
-            float mx[NR];
-#pragma unroll
-            for (int k = 0; k < NR; k++) {
-                mx[k] = ninf;
-#pragma unroll
-                for (int nt = 0; nt < 4; nt++) {
-                    const float f = qf[k] * (nt < 2 ? ks0 : ks1);
-                    const bool in = nt < 2 ? in0 : in1;
-#pragma unroll
-                    for (int c = 0; c < 2; c++) {
-                        const int key = key0 + 8 * nt + 2 * tq + c;
-                        const float z = SPLIT ? s[nt][c] + s[nt][c + 2] : s[nt][2 * k + c];
-                        p[k][2 * nt + c] = in && key < lim[k] ? z * f : ninf;
-                        mx[k] = fmaxf(mx[k], p[k][2 * nt + c]);
-                    }
-                }
-                mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
-                mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
-            }
-            // references: moved for the whole warp at once, seldom
-            const float vmax = fmaxf(vs0, vs1);  // 0 where there is no page
-            bool move = vmax > kAttnVRatio * vref;
-#pragma unroll
-            for (int k = 0; k < NR; k++) move |= mx[k] > ref[k] + kAttnRefMove;
-            if (__any_sync(0xffffffffu, move)) {
-                const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
-                const float vf = vnew > 0.0f ? vref / vnew : 0.0f;
-                vref = vnew;
-                float of[NR];
+                __syncwarp();
+                if (i + 2 < n_own) copy((i + 2) / 32 == i / 32 ? cur : nxt, i + 2, &a.tmap_k, my_k + st * C::kCodes, &k_bar[st]);
+                // scores in log2, masked
+                float p[NR][8];
+                float mx[NR];
 #pragma unroll
                 for (int k = 0; k < NR; k++) {
-                    float f = 1.0f;
-                    if (mx[k] > ref[k] + kAttnRefMove) {
-                        const float to = mx[k] - kAttnRefDrop;
-                        f = ex2(ref[k] - to);  // 0 for the first scores (ref = -inf)
-                        ref[k] = to;
+                    mx[k] = ninf;
+#pragma unroll
+                    for (int nt = 0; nt < 4; nt++) {
+                        const float f = qf[k] * (nt < 2 ? ks0 : ks1);
+                        const bool in = nt < 2 ? in0 : in1;
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const int key = key0 + 8 * nt + 2 * tq + c;
+                            const float z = SPLIT ? s[nt][c] + s[nt][c + 2] : s[nt][2 * k + c];
+                            p[k][2 * nt + c] = in && key < lim[k] ? z * f : ninf;
+                            mx[k] = fmaxf(mx[k], p[k][2 * nt + c]);
+                        }
                     }
-                    sum[k] *= f;
-                    of[k] = f * vf;
+                    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
+                    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
                 }
+                // references: moved for the whole warp at once, seldom
+                const float vmax = fmaxf(vs0, vs1);  // 0 where there is no page
+                bool move = vmax > kAttnVRatio * vref;
 #pragma unroll
-                for (int n = 0; n < D / 8; n++) {
-                    o[n][0] *= of[0], o[n][1] *= of[0];
-                    o[n][2] *= of[NR - 1], o[n][3] *= of[NR - 1];
-                }
-            }
-            const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f, r0 = vs0 * vinv, r1 = vs1 * vinv;
+                for (int k = 0; k < NR; k++) move |= mx[k] > ref[k] + kAttnRefMove;
+                if (__any_sync(0xffffffffu, move)) {
+                    const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
+                    const float vf = vnew > 0.0f ? vref / vnew : 0.0f;
+                    vref = vnew;
+                    float of[NR];
 #pragma unroll
-            for (int k = 0; k < NR; k++) {
-                const float base_ref = ref[k] == ninf ? 0.0f : ref[k];
-#pragma unroll
-                for (int n = 0; n < 8; n++) {
-                    const float e = ex2(p[k][n] - base_ref);
-                    sum[k] += e;
-                    p[k][n] = e * (n < 4 ? r0 : r1);
-                }
-            }
-            uint32_t pa[2][4];
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                if constexpr (SPLIT) {
-                    const float *pp = &p[0][4 * ks];
-                    const __half2 h0 = __floats2half2_rn(pp[0], pp[1]), h1 = __floats2half2_rn(pp[2], pp[3]);
-                    pa[ks][0] = h2u(h0);
-                    pa[ks][2] = h2u(h1);
-                    pa[ks][1] = pack_h2(pp[0] - __low2float(h0), pp[1] - __high2float(h0));
-                    pa[ks][3] = pack_h2(pp[2] - __low2float(h1), pp[3] - __high2float(h1));
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        pa[ks][k] = pack_h2(p[k][4 * ks], p[k][4 * ks + 1]);
-                        pa[ks][k + 2] = pack_h2(p[k][4 * ks + 2], p[k][4 * ks + 3]);
-                    }
-                }
-            }
-            if (!mbar_wait_bounded(v_bar, uint32_t(vc) & 1u)) dead = true;
-            dead = __any_sync(0xffffffffu, dead);
-            if (dead) break;
-            // O += P V
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                // e4m3: bytes of keys that are not there may be NaN, which 0 * NaN would keep
-                uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-                if constexpr (FMT != CPQ_KV_INT8) {
-#pragma unroll
-                    for (int n = 0; n < 4; n++)
-                        keep[n] = (ks ? in1 : in0) && key0 + 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1) < u.seq.kv ? ~0u : 0u;
-                }
-#pragma unroll
-                for (int at = 0; at < NA; at++) {
-                    uint4 vw[4];
-#pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        const int key = 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1);
-                        vw[n] = *reinterpret_cast<const uint4 *>(my_v + at * at_stride + ks * half_skip + key * 128 + ((gq ^ (key & 7)) << 4));
+                    for (int k = 0; k < NR; k++) {
+                        float f = 1.0f;
+                        if (mx[k] > ref[k] + kAttnRefMove) {
+                            const float to = mx[k] - kAttnRefDrop;
+                            f = ex2(ref[k] - to);  // 0 for the first scores (ref = -inf)
+                            ref[k] = to;
+                        }
+                        sum[k] *= f;
+                        of[k] = f * vf;
                     }
 #pragma unroll
-                    for (int wi = 0; wi < 4; wi++) {
-                        uint32_t w[4];
+                    for (int n = 0; n < D / 8; n++) {
+                        o[n][0] *= of[0], o[n][1] *= of[0];
+                        o[n][2] *= of[NR - 1], o[n][3] *= of[NR - 1];
+                    }
+                    if (SPLIT && i >= C::kFlush) {
+                        float4 *const acc = flushed();
+#pragma unroll 1
+                        for (int n = 0; n < D / 8; n++) attn_scale4(acc + 32 * n, of[0], of[NR - 1]);
+                    }
+                }
+                const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f, r0 = vs0 * vinv, r1 = vs1 * vinv;
+#pragma unroll
+                for (int k = 0; k < NR; k++) {
+                    const float base_ref = ref[k] == ninf ? 0.0f : ref[k];
+#pragma unroll
+                    for (int n = 0; n < 8; n++) {
+                        const float e = ex2(p[k][n] - base_ref);
+                        sum[k] += e;
+                        p[k][n] = e * (n < 4 ? r0 : r1);
+                    }
+                }
+                uint32_t pa[2][4];
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    if constexpr (SPLIT) {
+                        const float *pp = &p[0][4 * ks];
+                        const __half2 h0 = __floats2half2_rn(pp[0], pp[1]), h1 = __floats2half2_rn(pp[2], pp[3]);
+                        pa[ks][0] = h2u(h0);
+                        pa[ks][2] = h2u(h1);
+                        pa[ks][1] = pack_h2(pp[0] - __low2float(h0), pp[1] - __high2float(h0));
+                        pa[ks][3] = pack_h2(pp[2] - __low2float(h1), pp[3] - __high2float(h1));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 2; k++) {
+                            pa[ks][k] = pack_h2(p[k][4 * ks], p[k][4 * ks + 1]);
+                            pa[ks][k + 2] = pack_h2(p[k][4 * ks + 2], p[k][4 * ks + 3]);
+                        }
+                    }
+                }
+                if (!mbar_wait_bounded(v_bar, uint32_t(vc) & 1u)) dead = true;
+                dead = __any_sync(0xffffffffu, dead);
+                if (dead) break;
+                // O += P V
+#pragma unroll
+                for (int ks = 0; ks < 2; ks++) {
+                    // e4m3: bytes of keys that are not there may be NaN, which 0 * NaN would keep
+                    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+                    if constexpr (FMT != CPQ_KV_INT8) {
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            keep[n] = (ks ? in1 : in0) && key0 + 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1) < u.seq.kv ? ~0u : 0u;
+                    }
+#pragma unroll
+                    for (int at = 0; at < NA; at++) {
+                        uint4 vw[4];
 #pragma unroll
                         for (int n = 0; n < 4; n++) {
-                            w[n] = wi == 0 ? vw[n].x : wi == 1 ? vw[n].y : wi == 2 ? vw[n].z : vw[n].w;
-                            if constexpr (FMT != CPQ_KV_INT8) w[n] &= keep[n];
+                            const int key = 16 * ks + 2 * tq + (n & 1) + 8 * (n >> 1);
+                            vw[n] = *reinterpret_cast<const uint4 *>(my_v + at * at_stride + ks * half_skip + key * 128 + ((gq ^ (key & 7)) << 4));
                         }
-                        uint32_t b[4][2];
-                        codes_h2<FMT>(__byte_perm(w[0], w[1], 0x5140), b[0][0], b[1][0]);
-                        codes_h2<FMT>(__byte_perm(w[0], w[1], 0x7362), b[2][0], b[3][0]);
-                        codes_h2<FMT>(__byte_perm(w[2], w[3], 0x5140), b[0][1], b[1][1]);
-                        codes_h2<FMT>(__byte_perm(w[2], w[3], 0x7362), b[2][1], b[3][1]);
 #pragma unroll
-                        for (int n = 0; n < 4; n++) mma_f16(o[at * 16 + wi * 4 + n], pa[ks], b[n][0], b[n][1]);
+                        for (int wi = 0; wi < 4; wi++) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int n = 0; n < 4; n++) {
+                                w[n] = wi == 0 ? vw[n].x : wi == 1 ? vw[n].y : wi == 2 ? vw[n].z : vw[n].w;
+                                if constexpr (FMT != CPQ_KV_INT8) w[n] &= keep[n];
+                            }
+                            uint32_t b[4][2];
+                            codes_h2<FMT>(__byte_perm(w[0], w[1], 0x5140), b[0][0], b[1][0]);
+                            codes_h2<FMT>(__byte_perm(w[0], w[1], 0x7362), b[2][0], b[3][0]);
+                            codes_h2<FMT>(__byte_perm(w[2], w[3], 0x5140), b[0][1], b[1][1]);
+                            codes_h2<FMT>(__byte_perm(w[2], w[3], 0x7362), b[2][1], b[3][1]);
+#pragma unroll
+                            for (int n = 0; n < 4; n++) mma_f16(o[at * 16 + wi * 4 + n], pa[ks], b[n][0], b[n][1]);
+                        }
                     }
                 }
+                __syncwarp();
+                if (i + 1 < n_own) copy((i + 1) / 32 == i / 32 ? cur : nxt, i + 1, &a.tmap_v, my_v, v_bar);
             }
-            __syncwarp();
-            if (i + 1 < n_own) copy((i + 1) / 32 == i / 32 ? cur : nxt, i + 1, &a.tmap_v, my_v, v_bar);
+            if (!SPLIT || dead || i == n_own) break;
+            if constexpr (SPLIT) {
+                float4 *const acc = flushed();
+#pragma unroll
+                for (int n = 0; n < D / 8; n++) {
+                    attn_flush4(acc + 32 * n, i == C::kFlush, o[n][0], o[n][1], o[n][2], o[n][3]);
+                    o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+                }
+            }
         }
-
+        if (SPLIT && n_own > C::kFlush) {
+            const float4 *const acc = flushed();
+#pragma unroll
+            for (int n = 0; n < D / 8; n++) {
+                const float4 v = __ldcg(acc + 32 * n);
+                o[n][0] += v.x, o[n][1] += v.y, o[n][2] += v.z, o[n][3] += v.w;
+                if (n % 4 == 3) asm volatile("" ::: "memory");  // four loads in flight: no registers for more
+            }
+        }
         // join the warps: stats first, then the accumulators at the common reference. The next unit's first
         // copies of K go out meanwhile.
         const AttnUnit done = u;

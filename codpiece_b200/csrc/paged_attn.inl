@@ -17,10 +17,11 @@ static cpq_status kv_tensor_map(const cpq_kv_cache *c, const void *codes, CUtens
     return r == CUDA_SUCCESS ? CPQ_SUCCESS : fail(CPQ_ERR_CUDA, "cuTensorMapEncodeTiled (kv cache) failed (%d)", int(r));
 }
 
-// Workspace of a launch of `ctas` CTAs with `rows` rows per unit: partial accumulators, statistics, headers.
+// Workspace of a launch of `ctas` CTAs with `rows` rows per unit: partial accumulators, statistics, headers, flushed
+// accumulators.
 static size_t attn_ws_bytes(int ctas, int rows, int d) {
     const size_t slots = 2 * size_t(ctas);
-    return align_up(slots * rows * d * 4, 256) + align_up(slots * rows * 8, 256) + align_up(slots * 16, 256);
+    return align_up(slots * rows * d * 4, 256) + align_up(slots * rows * 8, 256) + align_up(slots * 16, 256) + size_t(ctas) * kAttnAcc * d;
 }
 
 static void attn_carve(AttnArgs &a, void *ws, int ctas, int rows, int d) {
@@ -31,6 +32,8 @@ static void attn_carve(AttnArgs &a, void *ws, int ctas, int rows, int d) {
     a.part_ml = reinterpret_cast<float2 *>(p);
     p += align_up(slots * rows * 8, 256);
     a.part_hdr = reinterpret_cast<int4 *>(p);
+    p += align_up(slots * 16, 256);
+    a.acc = reinterpret_cast<float4 *>(p);
 }
 
 template <int D, int ROWS>
@@ -109,9 +112,9 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     const bool split = q->type == CPQ_TYPE_F32;
     const int unit_rows = attn_rows(q, c, s->n_seqs);
     const bool tc = unit_rows == kTaRows;
-    // the units' tiles are counted in 32 bits
-    const int tile = tc ? kTaTile : kAttnTile;
-    const int64_t tiles = std::max<int64_t>(1, (int64_t(s->max_blocks) * c->block + tile - 1) / tile);
+    // the units' places (tiles, and those for beginning one) are counted in 32 bits
+    const int tile = tc ? kTaTile : kAttnTile, begin = tc ? kTaStart : DecCfg<128, true>::kStart;
+    const int64_t tiles = begin + std::max<int64_t>(1, (int64_t(s->max_blocks) * c->block + tile - 1) / tile);
     if ((rows / unit_rows + s->n_seqs * c->n_head_kv) > 2147483647 / tiles)
         return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: %lld rows over up to %lld keys are too many for one call", (long long)rows,
                     (long long)s->max_blocks * c->block);

@@ -74,6 +74,7 @@ struct TaInfo {
 
 template <int D, bool SPLIT> struct TaCfg {
     static constexpr int kVStages = SPLIT ? 2 : 4;
+    static constexpr int kFlush = SPLIT ? 6 : 32;         // tiles (16, 8 accumulation steps each) between flushes of O
     static constexpr int kBlock = kTaTile * 128;          // a 64-dim block of Q or K
     static constexpr int kVBlock = kTaQuarter * 128;      // of a V stage
     static constexpr int kK = kTaTile * D * 2, kV = kTaQuarter * D * 2, kQ = kTaRows * D * 2;
@@ -346,18 +347,22 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             auto scores = [&](int gi, bool fresh) {
                 if (!fresh && !tc_wait(pv_done, uint32_t(gi - 2) & 1u, abort_flag)) return false;
                 const uint32_t s = tmem + C::kColS + uint32_t(kTaTile) * uint32_t(gi & 1);
+                // fp32 q: the second terms come first, while the sums are small and lose next to nothing
 #pragma unroll
-                for (int b = 0; b < D / 64; b++) {
-                    if (!tc_wait(&k_full[b], uint32_t(gi) & 1u, abort_flag)) return false;
-                    tc_fence_after();
+                for (int term = SPLIT ? 1 : 0; term >= 0; term--) {
 #pragma unroll
-                    for (int x = 0; x < (SPLIT ? 8 : 4); x++) {
-                        const uint32_t at = uint32_t(b * (C::kBlock / 16) + 2 * (x & 3));
-                        if (b == 0 && x == 0) tc_mma1_ss<false>(s, q_lo, k_lo, idesc_s);
-                        else tc_mma1_ss<true>(s, q_lo + uint32_t((x >> 2) * (C::kQ / 16)) + at, k_lo + at, idesc_s);
+                    for (int b = 0; b < D / 64; b++) {
+                        if ((term || !SPLIT) && !tc_wait(&k_full[b], uint32_t(gi) & 1u, abort_flag)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const uint32_t at = uint32_t(b * (C::kBlock / 16) + 2 * x), q = q_lo + uint32_t(term * (C::kQ / 16)) + at;
+                            if (b == 0 && x == 0 && term == (SPLIT ? 1 : 0)) tc_mma1_ss<false>(s, q, k_lo + at, idesc_s);
+                            else tc_mma1_ss<true>(s, q, k_lo + at, idesc_s);
+                        }
+                        issued = true;
+                        if (term == 0) tc_commit1(&k_empty[b]);
                     }
-                    issued = true;
-                    tc_commit1(&k_empty[b]);
                 }
                 tc_commit1(&s_full[gi & 1]);
                 return true;
@@ -369,11 +374,12 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 tc_fence_after();
                 const uint32_t v = v_lo + uint32_t(st * (C::kV / 16));
                 const uint32_t p = tmem + C::kColS + uint32_t(kTaTile) * uint32_t(g & 1) + 32u * uint32_t(quarter);
-                if (fresh) tc_mma1_ts<false>(tmem + C::kColO, p, v, idesc_o);
-                else tc_mma1_ts<true>(tmem + C::kColO, p, v, idesc_o);
+                constexpr uint32_t first = SPLIT ? 8u : 0u;  // (second terms first here too)
+                if (fresh) tc_mma1_ts<false>(tmem + C::kColO, p + first, v, idesc_o);
+                else tc_mma1_ts<true>(tmem + C::kColO, p + first, v, idesc_o);
 #pragma unroll
                 for (int x = 1; x < (SPLIT ? 4 : 2); x++)
-                    tc_mma1_ts<true>(tmem + C::kColO, p + 8u * uint32_t(x >> 1) + 16u * uint32_t(x & 1), v + 128u * uint32_t(x & 1), idesc_o);
+                    tc_mma1_ts<true>(tmem + C::kColO, p + (x < 2 ? first : 0u) + 16u * uint32_t(x & 1), v + 128u * uint32_t(x & 1), idesc_o);
                 tc_commit1(&v_empty[st]);
                 return true;
             };
@@ -383,7 +389,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 n_units++;
                 for (int j = 0; ok && j < n; j++, g++) {
                     ok = (j + 1 == n || scores(g + 1, j == 0)) && tc_wait(&p_full[g & 1], uint32_t(g >> 1) & 1u, abort_flag);
-                    for (int x = 0; ok && x < 4; x++) ok = values(x, (j | x) == 0);
+                    for (int x = 0; ok && x < 4; x++) ok = values(x, (j % C::kFlush | x) == 0);
                     if (!ok) break;
                     tc_commit1(pv_done);
                 }
@@ -568,6 +574,13 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             const int lim = !there ? 0 : a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + i_tok + 1) : u.seq.kv;
             float ref = ninf, sum = 0.0f, vref = 0.0f;
             const int n = u.t1 - u.t0;
+            // half of the row's columns, by fours
+            auto flushed = [&]() {  // (from special registers: none held meanwhile)
+                uint32_t cta, thread;
+                asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+                asm volatile("mov.u32 %0, %%tid.x;" : "=r"(thread));
+                return a.acc + int64_t(cta) * (D / 4 * kTaRows) + ((thread - 128) >> 7) * (D / 8 * kTaRows) + (thread & 127);
+            };
             for (int j = 0; j < n; j++, g++) {
                 const int slot = g % kTaInfo;
                 const int key0 = (u.t0 + j) * kTaTile + kTaHalf * hf;
@@ -610,6 +623,20 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 soft_sync();
                 top = fmaxf(top, s_max[turn][hf ^ 1][rr]);
                 turn ^= 1;
+                if (j > 0 && j % C::kFlush == 0) {  // half of O's columns to the workspace; P(j) V begins a new O
+                    if (!__all_sync(0xffffffffu, tc_wait(pv_done, uint32_t(g - 1) & 1u, abort_flag))) ok = false;
+                    tc_fence_after();
+                    float4 *const acc = flushed();
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; c++) {
+                        uint32_t o[16];
+                        tmem_ld16_wait(tq + C::kColO + uint32_t(hf * (D / 2) + 16 * c), o);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            attn_flush4(acc + (4 * c + i) * kTaRows, j == C::kFlush, __uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                        __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    }
+                }
                 if (__any_sync(0xffffffffu, top > ref + kAttnRefMove || vmax > kAttnVRatio * vref)) {
                     const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
                     float f = vnew > 0.0f ? vref / vnew : 0.0f;
@@ -620,7 +647,12 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                         sum *= e;
                         f *= e;
                     }
-                    if (j > 0) {  // half of O's columns, once P(j - 1) V has been added
+                    if (j >= C::kFlush) {
+                        float4 *const acc = flushed();
+#pragma unroll 1
+                        for (int c = 0; c < D / 8; c++) attn_scale4(acc + c * kTaRows, f, f);
+                    }
+                    if (j % C::kFlush) {  // half of O's columns, once P(j - 1) V has been added
                         if (!__all_sync(0xffffffffu, tc_wait(pv_done, uint32_t(g - 1) & 1u, abort_flag))) ok = false;
                         tc_fence_after();
 #pragma unroll 1
@@ -679,6 +711,25 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             if (n > 1 && !__all_sync(0xffffffffu, tc_wait(pv_done, uint32_t(g - 2) & 1u, abort_flag))) ok = false;
             if (!__all_sync(0xffffffffu, tc_wait(pv_done, uint32_t(g - 1) & 1u, abort_flag))) ok = false;
             tc_fence_after();
+            if (n > C::kFlush) {  // what O held before
+                const float4 *const acc = flushed();
+#pragma unroll 1
+                for (int c = 0; c < D / 32; c++) {
+                    uint32_t o[16];
+                    const uint32_t at = tq + C::kColO + uint32_t(hf * (D / 2) + 16 * c);
+                    tmem_ld16_wait(at, o);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 v = __ldcg(acc + (4 * c + i) * kTaRows);
+                        o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) + v.x);
+                        o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) + v.y);
+                        o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) + v.z);
+                        o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) + v.w);
+                    }
+                    tmem_st16_async(at, o);
+                }
+                tmem_wait_st();
+            }
             s_max[turn][hf][rr] = sum;
             ok = !soft_any(!ok || *abort_flag);
             sum += s_max[turn][hf ^ 1][rr];

@@ -430,6 +430,109 @@ def test_attention_long(cuda, A, q_lens, kv_lens, heads, group, d, block, typ, f
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("typ,fmt", [("f32", "int8"), ("f32", "e4m3"), ("f16", "int8"), ("bf16", "e4m3")])
+def test_attention_many_rows_scales_and_pages_far_apart(cuda, A, typ, fmt):
+    """What test_attention_scales_and_scores_far_apart asks of few rows, with tiles of 128 rows."""
+    _attn_case(cuda, A, [40, 33], [500, 333], 1, 4, 128, 16, typ, fmt, spread=30.0)
+    _attn_case(cuda, A, [40, 33], [500, 333], 1, 4, 256, 32, typ, fmt, gain=12.0)
+    _attn_case(cuda, A, [50], [100], 1, 4, 256, 32, typ, fmt, scale=-0.1)
+    _attn_case(cuda, A, [50], [100], 1, 4, 128, 64, typ, fmt, scale=0.0)
+    _attn_case(cuda, A, [50], [100], 1, 3, 256, 128, typ, fmt, gain=1e-30)
+    _attn_case(cuda, A, [70, 1, 90], [1100, 700, 90], 1, 2, 256, 16, typ, fmt, bad_pages=True)
+    if typ == "f32":
+        _attn_case(cuda, A, [50], [100], 1, 2, 128, 32, typ, fmt, gain=1e30, scale=1e-31)
+
+
+@pytest.mark.parametrize("typ,fmt,d", [("f32", "int8", 256), ("f32", "e4m3", 128), ("bf16", "e4m3", 256)])
+def test_attention_one_row_each_with_pages_outside_the_pool(cuda, A, typ, fmt, d):
+    for block in (16, 32, 128):
+        _attn_case(cuda, A, [1, 1, 1, 1], [400, 164, 17, 290], 1, 2, d, block, typ, fmt, bad_pages=True)
+
+
+@pytest.mark.parametrize("typ,fmt,q_lens", [("f32", "int8", [1, 1]), ("bf16", "int8", [1, 1]), ("f32", "int8", [40, 9]), ("f16", "e4m3", [40, 9])])
+def test_attention_of_unaligned_views(cuda, A, typ, fmt, q_lens):
+    """Rows that begin off 16-byte boundaries give what aligned ones give."""
+    torch = cuda
+    dt = _dtype(torch, typ)
+    cache, _, _ = _pool(torch, A, 12, 2, 32, 128, fmt, seed=3)
+    table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+    start = torch.tensor([0, q_lens[0], sum(q_lens)], dtype=torch.int32, device="cuda")
+    kv = torch.tensor([190, 77], dtype=torch.int32, device="cuda")
+    t = sum(q_lens)
+    buf = torch.randn(t, 4 * 128 + 3, device="cuda").to(dt)
+    view = buf[:, 1:1 + 512].unflatten(-1, (4, 128))
+    to = torch.full((t, 4 * 128 + 3), 7.0, dtype=dt, device="cuda")
+    A.paged_attn(view, cache, table, start, kv, out=to[:, 1:513].unflatten(-1, (4, 128)))
+    want = A.paged_attn(view.contiguous(), cache, table, start, kv)
+    assert torch.equal(to[:, 1:513].unflatten(-1, (4, 128)), want)
+    assert (to[:, 0] == 7).all() and (to[:, 513:] == 7).all()
+
+
+@pytest.mark.parametrize("q_len", [1, 24])
+def test_attention_with_pages_of_scale_zero(cuda, A, q_len):
+    """A page of zeros has scale 0: its keys score 0 and its values add nothing."""
+    torch = cuda
+    cache, kvals, vvals = _pool(torch, A, 4, 1, 32, 128, "int8", seed=9)
+    cache.k_scale[2] = 0
+    cache.v_scale[2] = 0
+    q = torch.randn(q_len, 4, 128, device="cuda")
+    for order in ([0, 1, 2, 3], [2, 0, 1, 3], [2]):
+        table = torch.tensor([order], dtype=torch.int32, device="cuda")
+        kv = 32 * len(order) - 3
+        args = (q, cache, table, torch.tensor([0, q_len], dtype=torch.int32).cuda(), torch.tensor([kv], dtype=torch.int32).cuda())
+        got = A.paged_attn(*args)
+        ref = _dense(torch, A, q, cache, table, [0, q_len], [kv], True)
+        size = float(q.double().abs().max() * np.abs(kvals).max()) * 128 ** 0.5
+        assert ((got.double() - ref).abs() <= 2 * (size * (2.0 ** -22 + 10 * 2.0 ** -23) + 2.0 ** -20) * np.abs(vvals).max()).all()
+
+
+@pytest.mark.parametrize("q_len", [1, 8])
+def test_attention_of_1024_requests(cuda, A, q_len):
+    torch = cuda
+    n = 1024
+    cache, kvals, vvals = _pool(torch, A, 64, 2, 16, 128, "int8", seed=4)
+    g = torch.Generator().manual_seed(5)
+    kv = torch.randint(q_len, 100, (n,), generator=g).to(torch.int32)
+    table = torch.randint(0, 64, (n, 7), generator=g).to(torch.int32).cuda()  # requests share pages
+    start = torch.arange(n + 1, dtype=torch.int32, device="cuda") * q_len
+    q = torch.randn(n * q_len, 6, 128, generator=g).cuda()
+    got = A.paged_attn(q, cache, table, start, kv.cuda())
+    ref = _dense(torch, A, q, cache, table, start.tolist(), kv.tolist(), True)
+    size = float(q.double().abs().max() * np.abs(kvals).max()) * 128 ** 0.5
+    assert ((got.double() - ref).abs() <= 2 * (size * (2.0 ** -22 + 10 * 2.0 ** -23) + 2.0 ** -20) * np.abs(vvals).max()).all()
+    with pytest.raises(Exception):
+        A.paged_attn(q, cache, torch.zeros(1025, 7, dtype=torch.int32, device="cuda"),
+                     torch.zeros(1026, dtype=torch.int32, device="cuda"), torch.zeros(1025, dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("n,q_len,kv,d", [(60, 1, 60000, 128), (30, 1, 60000, 256), (40, 8, 20000, 128), (40, 8, 20000, 256)])
+def test_long_sums_do_not_drift(cuda, A, fmt, n, q_len, kv, d):
+    """All values positive: a sum that is cut off, not rounded, at each step falls short step by step. With V in
+    [0.5, 1] and equal weights a sum grows steadily, a step of 16 keys cuts less than 2^-23 of it, and over the
+    at most 128 steps between two flushes that is 128 * 2^-23 / 2 = 7.6e-6 of what the sum has become, plus 2^-20
+    for exponentials, terms of P and joins: 8.6e-6 at most. Unflushed, the expected shortfall of a share of 750
+    or 2500 steps is 1.6e-5 or 5e-5 (half of 2^-24 .. 2^-23 a step)."""
+    torch = cuda
+    block, heads, group = 64, 4, 6
+    pages = -(-kv // block)
+    cache = A.KvCache.empty(pages, heads, d, block, FMT[fmt])
+    g = torch.Generator("cuda").manual_seed(6)
+    x = torch.randint(64, 128, cache.v.shape, generator=g, device="cuda")
+    cache.v.copy_(x if fmt == "int8" else (x // 8).float())  # (8 to 15 are e4m3 values)
+    cache.v_scale.fill_(1.0 / 128 if fmt == "int8" else 1.0 / 16)
+    cache.k.zero_()
+    cache.k_scale.fill_(1.0)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(n, 1)  # all read the same pages
+    start = torch.arange(n + 1, dtype=torch.int32, device="cuda") * q_len
+    lens = torch.full((n,), kv, dtype=torch.int32, device="cuda")
+    q = torch.randn(n * q_len, heads * group, d, generator=g, device="cuda")
+    got = A.paged_attn(q, cache, table, start, lens, causal=False)
+    v = (cache.v.float() * cache.v_scale[0, 0]).double().transpose(0, 1).reshape(heads, -1, d)[:, :kv].mean(1)
+    ref = v.repeat_interleave(group, 0)
+    assert float((got.double() / ref - 1).abs().max()) <= 8.6e-6
+
+
 def test_attention_in_a_graph_and_on_another_stream(cuda, A):
     """Captured with its lengths on the device, replayed after they changed; two graphs replayed side by side."""
     torch = cuda
