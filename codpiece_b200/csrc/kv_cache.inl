@@ -98,7 +98,8 @@ extern "C" cpq_status cpq_kv_slots(const cpq_kv_slot_args *s, void *stream) {
     if (s->n_free > 0 && !s->free_pages) return fail(CPQ_ERR_INVALID_ARG, "kv_slots: null free_pages");
     SlotArgs a{s->ctx_len, s->new_len, s->n_seqs, s->table, s->table_stride, s->max_blocks, s->block,
                s->free_pages, s->n_free, s->taken, s->taken_out, s->seq_start, s->kv_len, s->pos, s->slot, s->n_rows};
-    // a row per thread; the scan, which every CTA repeats, takes longer than that
+    // a row per thread; the scan, which every CTA repeats, takes longer than that (300 requests, 60000 rows: 6.4 us,
+    // one CTA 72, eight times as many 6.2)
     const int64_t per_cta = 1024;
     int64_t ctas = s->taken_out == s->taken ? 1 : (s->n_rows + per_cta - 1) / per_cta;
     ctas = std::min<int64_t>(std::max<int64_t>(ctas, 1), sm_count(std::max(current_device(), 0)));
@@ -133,8 +134,9 @@ extern "C" cpq_status cpq_kv_append(const cpq_kv_cache *c, const cpq_tensor *k, 
     a.n_head = c->n_head_kv;
     a.d = c->head_dim;
     a.log_block = log_block(c->block);
-    // A group's runs are written one after another, so few rows get a CTA each; many rows are mostly
-    // insides of runs, whose CTAs would only look and leave.
+    // A group's runs are written one after another, so few rows get a CTA each (24 rows with the gather that follows:
+    // 8.0 us, groups of 32: 33); many rows are mostly insides of runs, whose CTAs would only look and leave (14000 rows:
+    // 60 us, groups of one: 260).
     const int64_t work = t * c->n_head_kv * 2, sms = sm_count(std::max(current_device(), 0));
     a.group = int(std::min<int64_t>(kAppendMaxGroup, std::max<int64_t>(1, work / (16 * sms))));
     const dim3 grid(unsigned((t + a.group - 1) / a.group), unsigned(c->n_head_kv), 2);

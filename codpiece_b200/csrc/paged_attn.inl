@@ -69,12 +69,23 @@ static cudaError_t launch_attn(const AttnArgs &a, bool tc, int fmt, int ctas, cu
     return tc ? launch_attn_tc<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st) : launch_attn_decode<D, CPQ_KV_E4M3, SPLIT>(a, ctas, st);
 }
 
-// The rows of a row tile: the decode kernel's while the sequences' query rows
-// (tokens x heads of a group) fill no more than one of its tiles on average,
-// else the tensor-core kernel's.
-static int attn_rows(const cpq_tensor *q, const cpq_kv_cache *c, int64_t n_seqs) {
-    const int few = q->type == CPQ_TYPE_F32 ? 8 : 16;
-    return q->ne[2] * (q->ne[1] / c->n_head_kv) <= few * n_seqs ? few : kTaRows;
+// The decode kernel or the tensor-core kernel. The first reads a sequence's keys
+// once per 8 or 16 query rows, the second once per 128 but begins late (some 15
+// us). Decode while sequences have at most two of its row tiles on average (24
+// heads over 4 of 256, us, decode : tensor core; fp32 1 request of 1 x 1000 keys
+// 13.6 : 27.5, 4 requests of 2 x 20000 73 : 99; bf16 16 of 4 x 4000 75 : 75, 4 of
+// 5 x 20000 78 : 82), and with more while the tables, which bound the keys, leave
+// at most 40 (row tile, 32 keys) per SM (1 request of 8 x 1000 16.9 : 29.7, 8 x
+// 8000 31 : 38, 32 x 1000 26 : 37; beyond, the tensor cores win: fp32 16 of 4 x 4000
+// 95 : 94, and 4 of 8 x 20001 81 where the other would read every key six times).
+static int attn_few(const cpq_tensor *q) { return q->type == CPQ_TYPE_F32 ? 8 : 16; }
+static bool attn_is_decode(const cpq_tensor *q, const cpq_kv_cache *c, int64_t n_seqs) {
+    return q->ne[2] * (q->ne[1] / c->n_head_kv) <= 2 * attn_few(q) * n_seqs;
+}
+static int attn_rows(const cpq_tensor *q, const cpq_kv_cache *c, int64_t n_seqs, int64_t keys, int sms) {
+    if (attn_is_decode(q, c, n_seqs)) return attn_few(q);
+    const int64_t tiles = q->ne[2] * (q->ne[1] / c->n_head_kv) / attn_few(q) + n_seqs, key_tiles = (keys + kAttnTile - 1) / kAttnTile;
+    return tiles <= 40 * sms && tiles * c->n_head_kv * key_tiles <= 40 * sms ? attn_few(q) : kTaRows;
 }
 
 }  // namespace cpq
@@ -82,7 +93,7 @@ static int attn_rows(const cpq_tensor *q, const cpq_kv_cache *c, int64_t n_seqs)
 extern "C" size_t cpq_paged_attn_workspace_size(const cpq_kv_cache *c, const cpq_tensor *q, int64_t n_seqs) {
     using namespace cpq;
     if (!c || !q || c->n_head_kv < 1) return 0;
-    return attn_ws_bytes(sm_count(std::max(current_device(), 0)), attn_rows(q, c, n_seqs), c->head_dim);
+    return attn_ws_bytes(sm_count(std::max(current_device(), 0)), attn_is_decode(q, c, n_seqs) ? attn_few(q) : kTaRows, c->head_dim);
 }
 
 extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c, const cpq_attn_seqs *s, float scale,
@@ -110,7 +121,8 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     if (rows > 2147483647 || c->n_pages * c->n_head_kv * c->block > 2147483647 || int64_t(s->max_blocks) * c->block > 2147483647)
         return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: more than 2^31 - 1 rows, cache rows or keys");
     const bool split = q->type == CPQ_TYPE_F32;
-    const int unit_rows = attn_rows(q, c, s->n_seqs);
+    const int ctas = sm_count(std::max(current_device(), 0));
+    const int unit_rows = attn_rows(q, c, s->n_seqs, int64_t(s->max_blocks) * c->block, ctas);
     const bool tc = unit_rows == kTaRows;
     // the units' places (tiles, and those for beginning one) are counted in 32 bits
     const int tile = tc ? kTaTile : kAttnTile, begin = tc ? kTaStart : DecCfg<128, true>::kStart;
@@ -119,10 +131,11 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
         return fail(CPQ_ERR_UNSUPPORTED, "paged_attn: %lld rows over up to %lld keys are too many for one call", (long long)rows,
                     (long long)s->max_blocks * c->block);
     if (!workspace) return fail(CPQ_ERR_NOT_INITIALIZED, "paged_attn: no workspace");
-    const int ctas = sm_count(std::max(current_device(), 0));
-    if (!aligned(workspace, 256) || workspace_bytes < attn_ws_bytes(ctas, unit_rows, c->head_dim))
-        return fail(CPQ_ERR_WORKSPACE, "paged_attn: workspace of %zu bytes, 256-byte aligned, needs %zu", workspace_bytes,
-                    attn_ws_bytes(ctas, unit_rows, c->head_dim));
+    const size_t need = cpq_paged_attn_workspace_size(c, q, s->n_seqs);
+    if (!aligned(workspace, 256) || workspace_bytes < need)
+        return fail(CPQ_ERR_WORKSPACE, "paged_attn: workspace of %zu bytes, 256-byte aligned, needs %zu", workspace_bytes, need);
+    if (q->data == out->data)
+        return fail(CPQ_ERR_INVALID_ARG, "paged_attn: out overlaps q (rows are read after others have been written)");
     AttnArgs a{};
     st = kv_tensor_map(c, c->k, &a.tmap_k);
     if (st == CPQ_SUCCESS) st = kv_tensor_map(c, c->v, &a.tmap_v);
@@ -154,7 +167,9 @@ extern "C" cpq_status cpq_paged_attn(const cpq_tensor *q, const cpq_kv_cache *c,
     a.causal = causal ? 1 : 0;
     a.scale_log2 = float(double(scale) * 1.4426950408889634);
     a.wide = wide_rows(q, 16) && wide_rows(out, 16) ? 1 : 0;
-    a.min_share = tc ? 1 : 4;  // short requests are spread wide: latency counts, joining costs little
+    // Short requests are spread wide, latency counts (1 x 1000 keys: 13.3 us, 16.4 with shares of 16 places; 8 x 1000
+    // on the tensor cores: 30, 56 with 6).
+    a.min_share = tc ? 1 : 4;
     attn_carve(a, workspace, ctas, unit_rows, c->head_dim);
     const cudaStream_t cs = static_cast<cudaStream_t>(stream);
     cudaError_t e;

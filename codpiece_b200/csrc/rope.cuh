@@ -132,6 +132,8 @@ template <typename T, int VEC> struct Vec<T, VEC, false> {
 // stores (finding each item by division took more instructions than the rest:
 // 8191 tokens x 40 heads of 128, bf16, 58 us). The first items' loads are
 // issued before the CTA makes its tokens' cos/sin table in shared memory.
+// Bounded by HBM, one read and one write of each element: that case takes 38.3
+// us, 4.4 TB/s (0.67 of a measured copy); 8 tokens x 28 heads 2.4 us, a launch.
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
     __shared__ __align__(16) float2 cs[kRopeMaxTok * kRopeMaxPairs];

@@ -235,3 +235,12 @@ def test_reference_slots_and_append_and_attention():
     assert np.allclose(o, [[1.0, 6.0]]) and math.isclose(lse[0], math.log(4.0))
     o, lse, _ = R.attention(np.zeros((3, 2)), k[:1], k[:1], 1.0, True)
     assert np.isneginf(lse[:2]).all() and (o[:2] == 0).all() and lse[2] == 0
+
+
+def test_paged_attn_refuses_out_in_place_of_q(L):
+    from codpiece_b200._lib import CpqAttnSeqs
+    q, c, s = tensor(256, 24, 3), cache(), CpqAttnSeqs()
+    out = tensor(256, 24, 3)  # the same address
+    for name, v in dict(seq_start=0x10, kv_len=0x20, table=0x30, table_stride=8, n_seqs=2, max_blocks=8).items():
+        setattr(s, name, v)
+    assert L.cpq_paged_attn(C.byref(q), C.byref(c), C.byref(s), 0.1, 1, C.byref(out), None, 0x80000, 1 << 30, None) == INVALID

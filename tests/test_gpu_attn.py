@@ -311,10 +311,23 @@ def _attn_case(torch, A, q_lens, kv_lens, heads, group, d, block, typ, fmt, caus
     out = torch.full((t, hq, d + 8), 5.0, dtype=dt, device="cuda")[..., :d]
     lse = torch.full((t, hq), 5.0, device="cuda")
     full = torch.tensor(np.concatenate([table, table], axis=1)).cuda()
-    A.paged_attn(q, cache, full[:, :width], torch.tensor(start).cuda(), torch.tensor(np.asarray(kv_lens, np.int32)).cuda(),
-                 causal=causal, out=out, lse=lse, scale=scale)
     sc = d ** -0.5 if scale is None else scale
-    ref, ref_lse, size = R.paged_attn(_np(q), kv, vv, table, start, kv_lens, sc, causal)
+    ref_all = R.paged_attn(_np(q), kv, vv, table, start, kv_lens, sc, causal)
+    # tables just wide enough, and so wide that more than a few rows go to the tensor-core kernel
+    for tab in (full[:, :width], torch.cat([full[:, :width], _no_pages(torch, n)], 1)):
+        out.fill_(5.0)
+        lse.fill_(5.0)
+        A.paged_attn(q, cache, tab, torch.tensor(start).cuda(), torch.tensor(np.asarray(kv_lens, np.int32)).cuda(),
+                     causal=causal, out=out, lse=lse, scale=scale)
+        _check_attn(torch, out, lse, ref_all, start, vv, d, typ)
+
+
+def _no_pages(torch, n):
+    return torch.full((n, 12000), -1, dtype=torch.int32, device="cuda")
+
+
+def _check_attn(torch, out, lse, ref_all, start, vv, d, typ):
+    (ref, ref_lse, size), dt = ref_all, out.dtype
     got, got_lse = _np(out), _np(lse)
     inside = int(start[-1])
     assert (got[inside:] == 5).all() and (got_lse[inside:] == 5).all(), "rows behind the last sequence"
@@ -456,6 +469,8 @@ def test_attention_of_unaligned_views(cuda, A, typ, fmt, q_lens):
     dt = _dtype(torch, typ)
     cache, _, _ = _pool(torch, A, 12, 2, 32, 128, fmt, seed=3)
     table = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)
+    if max(q_lens) > 1:
+        table = torch.cat([table, _no_pages(torch, 2)], 1)
     start = torch.tensor([0, q_lens[0], sum(q_lens)], dtype=torch.int32, device="cuda")
     kv = torch.tensor([190, 77], dtype=torch.int32, device="cuda")
     t = sum(q_lens)
@@ -477,7 +492,7 @@ def test_attention_with_pages_of_scale_zero(cuda, A, q_len):
     cache.v_scale[2] = 0
     q = torch.randn(q_len, 4, 128, device="cuda")
     for order in ([0, 1, 2, 3], [2, 0, 1, 3], [2]):
-        table = torch.tensor([order], dtype=torch.int32, device="cuda")
+        table = torch.cat([torch.tensor([order], dtype=torch.int32, device="cuda"), _no_pages(torch, 1)], 1)
         kv = 32 * len(order) - 3
         args = (q, cache, table, torch.tensor([0, q_len], dtype=torch.int32).cuda(), torch.tensor([kv], dtype=torch.int32).cuda())
         got = A.paged_attn(*args)
