@@ -78,22 +78,23 @@ constexpr int kAttnAcc = 512;    // bytes of acc per CTA and dim (128 rows, or 8
 // ---- the split ------------------------------------------------------------------
 
 struct AttnSeq {
-    int row0, q, kv;  // first token, tokens, keys
+    int row0, q, kv, seen;  // first token, tokens, keys, keys the table has blocks for
 };
 
 __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs &a, int s) {
     AttnSeq r;
     r.row0 = min(max(a.seq_start[s], 0), a.t);
     r.q = min(max(a.seq_start[s + 1], r.row0), a.t) - r.row0;
-    r.kv = int(min(int64_t(max(a.kv_len[s], 0)), int64_t(a.max_blocks) * a.block));
+    r.kv = max(a.kv_len[s], 0);
+    r.seen = min(r.kv, a.max_blocks * a.block);
     return r;
 }
 
 // Keys that the rows [r * rows, (r + 1) * rows) see together.
 __device__ __forceinline__ int attn_kv_end(const AttnSeq &s, int r, int rows, int group, int causal) {
-    if (!causal) return s.kv;
+    if (!causal) return s.seen;
     const int last = (min(s.q * group, (r + 1) * rows) - 1) / group;
-    return min(max(s.kv - s.q + last + 1, 0), s.kv);
+    return min(max(s.kv - s.q + last + 1, 0), s.seen);
 }
 
 __device__ __forceinline__ int attn_row_tiles(const AttnSeq &s, int rows, int group) { return (s.q * group + rows - 1) / rows; }

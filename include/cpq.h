@@ -516,7 +516,7 @@ typedef struct cpq_attn_seqs {
     const int32_t *table;     /* [n_seqs][table_stride] */
     int64_t table_stride;
     int64_t n_seqs;
-    int32_t max_blocks;       /* blocks a table row has; keys beyond them are not seen */
+    int32_t max_blocks;       /* blocks a table row has; keys beyond them are not seen (kv_len still places the rows) */
 } cpq_attn_seqs;
 
 /* out = softmax(scale * q K^T) V over the cached keys (their values code *

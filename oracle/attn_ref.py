@@ -152,7 +152,8 @@ def paged_attn(q, k_vals, v_vals, table, seq_start, kv_len, scale, causal):
     out, lse, size = np.full(q.shape, np.nan), np.full((t, hq), np.nan), 0.0
     for s in range(len(kv_len)):
         a, b = int(seq_start[s]), int(seq_start[s + 1])
-        m = min(max(int(kv_len[s]), 0), table.shape[1] * block)
+        kv = max(int(kv_len[s]), 0)
+        m = min(kv, table.shape[1] * block)  # keys behind the table's blocks are not seen
         ids = [int(table[s, j // block]) for j in range(m)]
         places = [j % block for j in range(m)]
         there = np.array([0 <= i < pages for i in ids], bool)
@@ -160,7 +161,7 @@ def paged_attn(q, k_vals, v_vals, table, seq_start, kv_len, scale, causal):
             for g in range(group):
                 qs = q[a:b, h * group + g]
                 for i in range(b - a):
-                    seen = min(max(m - (b - a) + i + 1, 0), m) if causal else m
+                    seen = min(max(kv - (b - a) + i + 1, 0), m) if causal else m
                     idx = [j for j in range(seen) if there[j]]
                     ks = np.array([k_vals[ids[j], h, places[j]] for j in idx]).reshape(len(idx), d)
                     vs = np.array([v_vals[ids[j], h, places[j]] for j in idx]).reshape(len(idx), d)

@@ -456,6 +456,25 @@ def test_attention_many_rows_scales_and_pages_far_apart(cuda, A, typ, fmt):
         _attn_case(cuda, A, [50], [100], 1, 2, 128, 32, typ, fmt, gain=1e30, scale=1e-31)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("typ,fmt,q_lens", [("f32", "int8", [1, 2]), ("bf16", "e4m3", [1, 2]), ("f32", "e4m3", [60, 30]), ("f16", "int8", [60, 30])])
+def test_attention_with_tables_shorter_than_the_lengths(cuda, A, typ, fmt, q_lens, causal):
+    """A row's limit goes by kv_len; keys in blocks that the table does not have are not seen."""
+    torch = cuda
+    dt = _dtype(torch, typ)
+    for block, cols, heads in ((16, 5, 1), (32, 3, 2), (64, 1, 2)):
+        cache, kv, vv = _pool(torch, A, 2 * cols, heads, block, 128, fmt, seed=8)
+        table = torch.randperm(2 * cols, generator=torch.Generator().manual_seed(3)).to(torch.int32).view(2, cols)
+        lens = [block * cols + 7, 2 ** 31 - 1]
+        start = np.concatenate([[0], np.cumsum(q_lens)]).astype(np.int32)
+        q = torch.randn(int(start[-1]), 3 * heads, 128, generator=torch.Generator().manual_seed(4)).to(dt).cuda()
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        A.paged_attn(q, cache, table.cuda(), torch.tensor(start).cuda(), torch.tensor(lens, dtype=torch.int32).cuda(),
+                     causal=causal, out=out, lse=lse)
+        ref = R.paged_attn(_np(q), kv, vv, table.numpy(), start, lens, 128 ** -0.5, causal)
+        _check_attn(torch, out, lse, ref, start, vv, 128, typ)
+
+
 @pytest.mark.parametrize("typ,fmt,d", [("f32", "int8", 256), ("f32", "e4m3", 128), ("bf16", "e4m3", 256)])
 def test_attention_one_row_each_with_pages_outside_the_pool(cuda, A, typ, fmt, d):
     for block in (16, 32, 128):
