@@ -24,7 +24,7 @@ namespace cpq {
 constexpr int kRopeMaxPairs = 128;
 constexpr int kRopeMaxTensors = 4;
 constexpr int kRopeThreads = 256;
-constexpr int kRopeMaxTok = 4;  // tokens of a CTA
+constexpr int kRopeMaxTok = 8;  // tokens of a CTA
 
 // Division of n < 2^31 by a divisor known on the host (round-up method:
 // q = (umulhi(n, m) + n) >> s).
@@ -132,13 +132,16 @@ template <typename T, int VEC> struct Vec<T, VEC, false> {
 // stores (finding each item by division took more instructions than the rest:
 // 8191 tokens x 40 heads of 128, bf16, 58 us). The first items' loads are
 // issued before the CTA makes its tokens' cos/sin table in shared memory.
-// Bounded by HBM, one read and one write of each element: that case takes 38.3
-// us, 4.4 TB/s (0.67 of a measured copy); 8 tokens x 28 heads 2.4 us, a launch.
+// (Four items in flight instead of two: interleaved fp32 88 us instead of 69, bf16
+// 36.6 instead of 38.7.)
+// Bounded by HBM, one read and one write of each element, and each CTA's
+// beginning: that case takes 36.6 us, 4.6 TB/s (0.7 of a measured copy), with
+// halves in fp32 58.7 us, 5.7 TB/s; 8 tokens x 28 heads 2.3 us, a launch.
 template <typename T, int VEC, bool HALF>
 __global__ void __launch_bounds__(kRopeThreads, 4) rope_kernel(const __grid_constant__ RopeArgs a) {
     __shared__ __align__(16) float2 cs[kRopeMaxTok * kRopeMaxPairs];
     using V = Vec<T, VEC>;
-    constexpr int NV = HALF ? 2 : 1, kBatch = HALF ? 2 : 4;
+    constexpr int NV = HALF ? 2 : 1, kBatch = HALF || sizeof(T) == 4 ? 2 : 4;  // items of a thread in flight
     constexpr int kPairs = HALF ? VEC : VEC / 2;  // of an item
     const int half_n = a.n_dims / 2, row = (half_n + 1) & ~1;
     const int64_t tok0 = int64_t(blockIdx.x) * a.tok_per_cta;

@@ -143,15 +143,16 @@ extern "C" cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *con
     a.pair_items = half ? rope->n_dims / 2 / width : (rope->n_dims + width - 1) / width;
     a.items = a.pair_items + (copy ? int(d - (half ? rope->n_dims : a.pair_items * width)) / width : 0);
     if (t > 2147483647) return fail(CPQ_ERR_UNSUPPORTED, "rope: %lld tokens", (long long)t);
-    // a CTA takes one token's heads, or several tokens' once that still gives every SM its CTAs (40 heads of 128, bf16,
-    // us: 8191 tokens 38 with four, 54 with one; 1480 tokens 9.0 with two, 10.8 with one, 9.5 with four); few tokens
+    // a CTA takes as many tokens' heads (up to kRopeMaxTok) as make whole waves of four CTAs per SM (40 heads of 128,
+    // bf16, us: 8191 tokens 36.6 with seven in two waves, 38.3 with four in 3.5, 54 with one; halves 34.5 : 38.3); few tokens
     // share their heads out over as many CTAs as fill the GPU, down to about one item per thread (8 tokens x 28 heads:
     // 2.4, a CTA per token 4.0)
     const int heads = a.head0[n], least = std::min(heads, (kRopeThreads + a.items - 1) / a.items);
     const int64_t sms = sm_count(std::max(current_device(), 0));
     const int64_t groups = std::max<int64_t>(1, std::min<int64_t>(heads / least, 2 * sms / t));
     a.heads_per_cta = int((heads + groups - 1) / groups);
-    a.tok_per_cta = t >= 20 * sms ? 4 : t >= 10 * sms ? 2 : 1;
+    const int64_t waves = (t + kRopeMaxTok * 4 * sms - 1) / (kRopeMaxTok * 4 * sms);
+    a.tok_per_cta = int((t + waves * 4 * sms - 1) / (waves * 4 * sms));
     a.t = t;
     a.by_items = FastDiv(uint32_t(a.items));
     a.step = std::max(1, kRopeThreads / a.items);
