@@ -341,13 +341,15 @@ struct AppendArgs {
 // a new page), the rows held before coded again if the scale rose, the new
 // rows' codes. Holding the rows in registers between the two passes instead
 // spilled and left an SM too few runs in flight (14080 rows x 8 heads of 128,
-// bf16, pages of 32: 42 us). That case takes 35 us now (2.4 TB/s), with fp32 rows
-// 37 (3.9 TB/s, 0.6 of a measured copy): the two passes over a run in shared
-// memory, a dozen instructions a value, bound it, not its bytes.
+// bf16, pages of 32: 42 us). That case takes 34 us now (2.5 TB/s), with fp32 rows
+// 36 (4.0 TB/s, 0.6 of a measured copy): what a CTA does before its copies and the
+// two passes over a run in shared memory bound it (68 % of issue slots), not its
+// bytes. 64 threads per 8 KB: with twice as many 39 us, with half 36 (fp32 57, 34).
+// 40 registers instead of 48 (a few spilled outside the loops): 3 to 9 % less.
 constexpr int kAppendMaxGroup = 32;
 
 template <typename T, bool WIDE, int FMT>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 6) kv_append_kernel(const __grid_constant__ AppendArgs a) {
     extern __shared__ __align__(128) uint8_t s_rows[];
     __shared__ float s_max[2][kAppendThreads / 32];
     __shared__ int64_t s_slot[1 + kAppendMaxGroup + 128];  // of the row before the group, the group, a page's rows behind it
