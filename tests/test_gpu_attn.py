@@ -567,6 +567,28 @@ def test_long_sums_do_not_drift(cuda, A, fmt, n, q_len, kv, d):
     assert float((got.double() / ref - 1).abs().max()) <= 8.6e-6
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("q_len,wide", [(2, False), (60, True)])
+def test_attention_rows_with_nan_and_infinity_spoil_no_others(cuda, A, typ, q_len, wide):
+    torch = cuda
+    dt = _dtype(torch, typ)
+    cache, _, _ = _pool(torch, A, 40, 2, 32, 128, "int8", seed=7)
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40)
+    if wide:  # the kernel for many rows
+        table = torch.cat([table, _no_pages(torch, 1)], 1)
+    start, kv = torch.tensor([0, q_len], dtype=torch.int32).cuda(), torch.tensor([1270], dtype=torch.int32).cuda()
+    q = torch.randn(q_len, 8, 128, device="cuda").to(dt)
+    clean = A.paged_attn(q, cache, table, start, kv)
+    bad = q.clone()
+    bad[0, 1, 5] = float("nan")
+    bad[1, 6, 7] = float("inf")
+    got = A.paged_attn(bad, cache, table, start, kv)
+    keep = torch.ones(q_len, 8, dtype=torch.bool, device="cuda")
+    keep[0, 1] = keep[1, 6] = False
+    assert torch.equal(got[keep], clean[keep])
+    assert not torch.isfinite(got[0, 1]).any()
+
+
 def test_attention_in_a_graph_and_on_another_stream(cuda, A):
     """Captured with its lengths on the device, replayed after they changed; two graphs replayed side by side."""
     torch = cuda
