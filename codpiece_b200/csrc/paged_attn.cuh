@@ -11,13 +11,19 @@
 // tensor cores with the page scales applied in fp32 around them. q is brought
 // to fp16 by a power of two per row: one term holds an fp16 or bf16 value
 // exactly; an fp32 value takes two (22 bits, the second the rounding error of
-// the first). Probabilities enter the second product the same way: one fp16
-// term for 16-bit outputs, two for fp32. The softmax reference of a row is
-// set 2 (in log2) under a maximum and moves when a score exceeds it by more than
-// 12, so probabilities lie in [0, 2^12] and it moves once or twice in a row's
-// life (with 8 and 11 some row of a warp moved in every second or third tile,
-// and each time O is rescaled); a page's v_scale enters as its ratio to a
-// reference scale, which moves when a ratio exceeds 8. Sums are fp32.
+// the first). What enters the second product is a key's contribution P_j =
+// 2^(z_j - ref) * v_scale[page(j)] / unit, the same way: one fp16 term for 16-bit
+// outputs, two for fp32. The unit is a power of two near the first pages' scales,
+// ref a whole number per row that follows the row's largest contribution, not its
+// largest score: set so that this one lies in [2^5, 2^6), and moved when one would
+// pass 2^15. So a row keeps 2^-30 of its largest contribution (half a step of
+// fp16's smallest numbers) however far the scales of pages lie apart that it
+// does not see or gives no weight. (With a unit that followed the largest scale
+// of the tile, one page of 10^6 times the other scales left the others five
+// bits.) ref moves once or twice in a row's life; set only 3 (in log2) under its
+// limit, some row of a warp moved it in every second or third tile, and each
+// time O is rescaled. The row sums of 2^(z_j - ref) are fp32, which has room for
+// scales 2^60 to either side of the first pages'. Sums are fp32.
 // The tensor cores cut a sum's bits below fp32 off instead of rounding them, so
 // every accumulation step loses a little on the same side (fp32 q, a row over
 // 9000 keys, 1130 steps: 1.6e-5 off in the 2-norm; 272 steps: 3.5e-6). After
@@ -288,14 +294,33 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-constexpr float kAttnRefDrop = 2.0f;    // the reference lies this far under the maximum it was set by
-constexpr float kAttnRefMove = 12.0f;   // and moves when a score is this far above it
-constexpr float kAttnVRatio = 8.0f;     // the v_scale reference moves when a page's scale is this many times it
+constexpr float kAttnRefDrop = 5.0f;    // a row's largest contribution is 2^5 .. 2^6 when its reference is set
+constexpr float kAttnRefMove = 15.0f;   // and the reference moves when one would pass 2^15
+constexpr float kAttnVLow = -64.0f;     // scales under 2^-64 units count as 2^-64 for the reference (row sums stay under 2^110)
+constexpr float kAttnVHigh = 0x1p90f;   // scales above this many units change the unit
 constexpr float kLn2 = 0.69314718055994531f;
 
-// lse of a row from its reference (log2) and sum.
+// 1 / unit for pages with scales up to vmax: a power of two, 0 while all are 0.
+__device__ __forceinline__ float attn_v_unit(float vmax) {
+    const int e = int(__float_as_uint(vmax) >> 23) - 127;
+    return vmax > 0.0f ? attn_exp2i(-min(max(e, -126), 126)) : 0.0f;
+}
+// The unit again.
+__device__ __forceinline__ float attn_v_scale(float vinv) { return vinv > 0.0f ? 1.0f / vinv : 0.0f; }
+// log2 of a page's scale in units, as the reference counts it.
+__device__ __forceinline__ float attn_v_log(float r) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(r));
+    return fmaxf(y, kAttnVLow);
+}
+
+// lse of a row from its reference (log2, whole) and sum, whose exponent is taken apart: the logarithm of a large sum
+// has a large rounding error.
 __device__ __forceinline__ float attn_lse(float ref, float sum) {
-    return sum == 0.0f ? __int_as_float(0xff800000) : (ref + __log2f(sum)) * kLn2;
+    if (sum == 0.0f) return __int_as_float(0xff800000);
+    const int bits = __float_as_int(sum), e = (bits >> 23) - 127;
+    if (bits < 0 || e == 128) return ref + sum;  // NaN, infinity
+    return ((ref + float(e)) + __log2f(__int_as_float((bits & 0x7fffff) | 0x3f800000))) * kLn2;
 }
 
 // ---- few query rows: mma.sync tiles, one key tile per warp -------------------------
@@ -344,10 +369,9 @@ template <int D, bool SPLIT> struct DecCfg {
     static constexpr int kQOff = kVOff + kWarps * kCodes;
     static constexpr int kRedBytes = 4 * kRows * D * 4;          // four warps' accumulators, in V's place
     static constexpr int kBarOff = kQOff + D / 16 * 512;
-    // stats (reference, sum) per warp and row, v reference per warp, row factors
+    // stats (reference, sum) per warp and row, row factors
     static constexpr int kStatOff = kBarOff + kWarps * 3 * 8;
-    static constexpr int kVStatOff = kStatOff + kWarps * 16 * 8;
-    static constexpr int kRowOff = kVStatOff + kWarps * 4;
+    static constexpr int kRowOff = kStatOff + kWarps * 16 * 8;
     static constexpr int kPlanOff = kRowOff + 16 * 4;
     static constexpr int kSmem = kPlanOff + int(sizeof(AttnPlan)) + 1024;
     static_assert(kRedBytes <= kWarps * kCodes, "the accumulators fit in V's place");
@@ -388,7 +412,6 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
     uint4 *sq = reinterpret_cast<uint4 *>(smem + C::kQOff);
     float *red = reinterpret_cast<float *>(smem + C::kVOff);
     float2 *stat = reinterpret_cast<float2 *>(smem + C::kStatOff);  // [warp][16 rows]: reference, sum
-    float *vstat = reinterpret_cast<float *>(smem + C::kVStatOff);
     float *rowf = reinterpret_cast<float *>(smem + C::kRowOff);     // [row]: 2^-shift of its q
     AttnPlan &plan = *reinterpret_cast<AttnPlan *>(smem + C::kPlanOff);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -535,7 +558,7 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
             qf[k] = rowf[gq + 8 * k] * a.scale_log2;
             lim[k] = a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + row / a.group + 1) : u.seq.kv;
         }
-        float vref = 0.0f;
+        float vinv = 0.0f;  // 1 / unit
         for (int i = 0;;) {
             const int stop = SPLIT ? min(n_own, i + C::kFlush) : n_own;
             for (; i < stop; i++, kc++, vc++) {
@@ -580,12 +603,20 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
                 }
                 __syncwarp();
                 if (i + 2 < n_own) copy((i + 2) / 32 == i / 32 ? cur : nxt, i + 2, &a.tmap_k, my_k + st * C::kCodes, &k_bar[st]);
-                // scores in log2, masked
+                float vf = 1.0f;  // old unit / new unit
+                const float vmax = fmaxf(vs0, vs1);  // 0 where there is no page
+                if (vinv == 0.0f || vmax * vinv > kAttnVHigh) {
+                    const float old = vinv;
+                    vinv = attn_v_unit(vmax);
+                    if (old > 0.0f) vf = vinv / old;
+                }
+                const float l0 = attn_v_log(vs0 * vinv), l1 = attn_v_log(vs1 * vinv);
+                // scores in log2, masked; the largest contribution
                 float p[NR][8];
-                float mx[NR];
+                float top[NR];
 #pragma unroll
                 for (int k = 0; k < NR; k++) {
-                    mx[k] = ninf;
+                    float mx[2] = {ninf, ninf};
 #pragma unroll
                     for (int nt = 0; nt < 4; nt++) {
                         const float f = qf[k] * (nt < 2 ? ks0 : ks1);
@@ -595,27 +626,24 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
                             const int key = key0 + 8 * nt + 2 * tq + c;
                             const float z = SPLIT ? s[nt][c] + s[nt][c + 2] : s[nt][2 * k + c];
                             p[k][2 * nt + c] = in && key < lim[k] ? z * f : ninf;
-                            mx[k] = fmaxf(mx[k], p[k][2 * nt + c]);
+                            mx[nt >> 1] = fmaxf(mx[nt >> 1], p[k][2 * nt + c]);
                         }
                     }
-                    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 1));
-                    mx[k] = fmaxf(mx[k], __shfl_xor_sync(0xffffffffu, mx[k], 2));
+                    top[k] = fmaxf(mx[0] + l0, mx[1] + l1);
+                    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1));
+                    top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 2));
                 }
                 // references: moved for the whole warp at once, seldom
-                const float vmax = fmaxf(vs0, vs1);  // 0 where there is no page
-                bool move = vmax > kAttnVRatio * vref;
+                bool move = vf != 1.0f;
 #pragma unroll
-                for (int k = 0; k < NR; k++) move |= mx[k] > ref[k] + kAttnRefMove;
+                for (int k = 0; k < NR; k++) move |= top[k] - ref[k] > kAttnRefMove;  // (exact for scores of any size; NaN before the first)
                 if (__any_sync(0xffffffffu, move)) {
-                    const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
-                    const float vf = vnew > 0.0f ? vref / vnew : 0.0f;
-                    vref = vnew;
                     float of[NR];
 #pragma unroll
                     for (int k = 0; k < NR; k++) {
                         float f = 1.0f;
-                        if (mx[k] > ref[k] + kAttnRefMove) {
-                            const float to = mx[k] - kAttnRefDrop;
+                        if (top[k] - ref[k] > kAttnRefMove) {
+                            const float to = floorf(top[k]) - kAttnRefDrop;
                             f = ex2(ref[k] - to);  // 0 for the first scores (ref = -inf)
                             ref[k] = to;
                         }
@@ -633,7 +661,7 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
                         for (int n = 0; n < D / 8; n++) attn_scale4(acc + 32 * n, of[0], of[NR - 1]);
                     }
                 }
-                const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f, r0 = vs0 * vinv, r1 = vs1 * vinv;
+                const float r0 = vs0 * vinv, r1 = vs1 * vinv;
 #pragma unroll
                 for (int k = 0; k < NR; k++) {
                     const float base_ref = ref[k] == ninf ? 0.0f : ref[k];
@@ -737,7 +765,6 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
             sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
             if (tq == 0) stat[warp * 16 + gq + 8 * k] = make_float2(ref[k], sum[k]);
         }
-        if (lane == 0) vstat[warp] = vref;
         __syncthreads();
         float top[NR], all[NR];
 #pragma unroll
@@ -760,7 +787,7 @@ __global__ void __launch_bounds__(DecCfg<D, SPLIT>::kThreads, 1) attn_decode_ker
             if ((warp >> 2) == r) {
 #pragma unroll
                 for (int k = 0; k < NR; k++) {
-                    const float f = ex2(ref[k] - (top[k] == ninf ? 0.0f : top[k])) * vref;
+                    const float f = ex2(ref[k] - (top[k] == ninf ? 0.0f : top[k])) * attn_v_scale(vinv);
 #pragma unroll
                     for (int i = 0; i < D / 8; i++) {
                         float2 *to = reinterpret_cast<float2 *>(mine + (i * kRows + gq + 8 * k) * 8 + 2 * tq);

@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(q_full);
             }
             const int lim = !there ? 0 : a.causal ? min(u.seq.kv, u.seq.kv - u.seq.q + i_tok + 1) : u.seq.kv;
-            float ref = ninf, sum = 0.0f, vref = 0.0f;
+            float ref = ninf, sum = 0.0f, vinv = 0.0f;  // (1 / unit)
             const int n = u.t1 - u.t0;
             // half of the row's columns, by fours
             auto flushed = [&]() {  // (from special registers: none held meanwhile)
@@ -600,6 +600,12 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                 float vmax = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) vmax = fmaxf(vmax, in.vs[i]);  // 0 where there is no page
+                float vf = 1.0f;  // old unit / new unit, the same for all rows
+                if (vinv == 0.0f || vmax * vinv > kAttnVHigh) {
+                    const float old = vinv;
+                    vinv = attn_v_unit(vmax);
+                    if (old > 0.0f) vf = vinv / old;
+                }
                 // keys past the row's limit or without a page: -inf in S
                 const bool clear = key0 + kTaHalf <= lim && min(min(in.row[4 * hf], in.row[4 * hf + 1]), min(in.row[4 * hf + 2], in.row[4 * hf + 3])) >= 0;
                 if (!__all_sync(0xffffffffu, clear)) {
@@ -614,7 +620,9 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                     }
                     tmem_wait_st();
                 }
-                // the maximum of the scores (log2)
+                // the largest contribution (log2, from the reference on, rounded as P's exponents below)
+                float base = ref == ninf ? 0.0f : ref;
+                const float limit = ref == ninf ? ninf : kAttnRefMove;
                 float top = ninf;
 #pragma unroll 1
                 for (int c = 0; c < 2; c++) {
@@ -623,8 +631,9 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                     float m[4];
 #pragma unroll
                     for (int i = 0; i < 32; i++) m[i >> 3] = (i & 7) == 0 ? z[i] : fmaxf(m[i >> 3], z[i]);
-                    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]) * ta_factor(in.ks[4 * hf + 2 * c] * qf),
-                                           fmaxf(m[2], m[3]) * ta_factor(in.ks[4 * hf + 2 * c + 1] * qf)));
+                    const int i = 4 * hf + 2 * c;
+                    top = fmaxf(top, fmaxf(__fmaf_rn(fmaxf(m[0], m[1]), ta_factor(in.ks[i] * qf), -base) + attn_v_log(in.vs[i] * vinv),
+                                           __fmaf_rn(fmaxf(m[2], m[3]), ta_factor(in.ks[i + 1] * qf), -base) + attn_v_log(in.vs[i + 1] * vinv)));
                 }
                 s_max[turn][hf][rr] = top;
                 soft_sync();
@@ -644,13 +653,11 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                                         __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
                     }
                 }
-                if (__any_sync(0xffffffffu, top > ref + kAttnRefMove || vmax > kAttnVRatio * vref)) {
-                    const float vnew = vmax > kAttnVRatio * vref ? vmax : vref;
-                    float f = vnew > 0.0f ? vref / vnew : 0.0f;
-                    vref = vnew;
-                    if (top > ref + kAttnRefMove) {
-                        const float to = top - kAttnRefDrop, e = ex2(ref - to);
-                        ref = to;
+                if (__any_sync(0xffffffffu, top > limit || vf != 1.0f)) {
+                    float f = vf;
+                    if (top > limit) {
+                        const float to = base + (floorf(top) - kAttnRefDrop), e = ex2(ref - to);
+                        ref = base = to;
                         sum *= e;
                         f *= e;
                     }
@@ -674,8 +681,6 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
                         }
                     }
                 }
-                const float base = ref == ninf ? 0.0f : ref;
-                const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
                 const uint64_t nbase = f2_pack(-base, -base);
                 uint64_t part[2] = {0, 0};  // (two zeros each)
 #pragma unroll 1
@@ -743,7 +748,7 @@ __global__ void __launch_bounds__(kTaThreads, 1) attn_tc_kernel(const __grid_con
             turn ^= 1;
             const bool whole = u.t0 == 0 && u.t1 == u.n;
             const int slot = attn_slot(u);
-            const float f = whole ? vref * attn_inverse(sum) : vref;
+            const float f = whole ? attn_v_scale(vinv) * attn_inverse(sum) : attn_v_scale(vinv);
 #pragma unroll 1
             for (int c = 0; c < D / 64; c++) {
                 float o[32];

@@ -529,7 +529,10 @@ typedef struct cpq_attn_seqs {
  * ([tokens][n_head] F32, or NULL) receives log sum exp of the scaled scores
  * (-inf for a row that sees none). out must not overlap q. Sums are fp32; with
  * F32 q the products carry 22 bits, with F16 and BF16 probabilities enter the
- * second product in fp16. workspace: at least cpq_paged_attn_workspace_size
+ * second product in fp16. A key's weight times its v_scale is held no finer
+ * than 2^-30 of the row's largest; that holds while the v_scales of a
+ * sequence's pages lie within 2^60 of one another, beyond it pages of the
+ * smaller scales may vanish. workspace: at least cpq_paged_attn_workspace_size
  * bytes, 256-byte aligned, any contents, in use until the call has run: calls
  * (and captured graphs) that may overlap on the GPU need workspaces of their
  * own. */
