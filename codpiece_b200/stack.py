@@ -383,13 +383,18 @@ class Stack:
         attn.paged_attn(q, cache, core.table, self.slots.seq_start, self.slots.kv_len, out=heads(self.ab, self.hp.n_head))
 
     def capture(self) -> None:
-        """Capture step_body() into a CUDA graph (run one eager step first to warm up)."""
+        """Capture step_body() into a CUDA graph (one eager step runs first to warm up: with an
+        attention core a step of no tokens, which leaves its cache and length as they are)."""
+        if self.attn is not None:
+            self.new_len.zero_()
         s = torch.cuda.Stream(device=self.dev)
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
             self.step_body()
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize(self.dev)
+        if self.attn is not None:
+            self.new_len.fill_(self.m)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.step_body()

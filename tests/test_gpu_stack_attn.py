@@ -126,3 +126,37 @@ def test_stack_refuses_what_the_core_does_not_run(cuda):
         stack.Stack(tp.HP_BENCH_27B, n_layer=2, m=1, head=False, attn_core=core)
     with pytest.raises(ValueError):
         stack.Stack(tp.HP_BENCH_27B, n_layer=1, m=1, head=False, attn_core=core, use_trunk=True)
+
+
+@pytest.mark.parametrize("m", [1, 4])
+def test_capture_in_mid_sequence_caches_nothing(cuda, m):
+    """What capture() runs to warm up is no token of the sequence: length, pages, codes and scales stay, and the replayed
+    steps go on where the eager ones ended."""
+    torch = cuda
+    from codpiece_b200 import attn, stack, tp
+
+    xs = torch.randn(5, m, 5120, device="cuda", generator=torch.Generator("cuda").manual_seed(4))
+    outs = []
+    for captured in (False, True):
+        core = _core(stack, tp, attn, 1, max_ctx=64, block=16)
+        s = stack.Stack(tp.HP_BENCH_27B, n_layer=1, m=m, seed=5, head=False, attn_core=core)
+        for x in xs[:2]:
+            s.h.copy_(x)
+            s.step_body()
+        if captured:
+            c = core.caches[0]
+            state = [core.ctx, core.taken, core.table, c.k, c.v, c.k_scale, c.v_scale]
+            before = [t.clone() for t in state]
+            s.h.copy_(100 * xs[2])
+            s.capture()
+            for t, b in zip(state, before):
+                assert torch.equal(t.view(torch.uint8), b.view(torch.uint8))
+        got = []
+        for x in xs[2:]:
+            s.h.copy_(x)
+            s.replay() if captured else s.step_body()
+            got.append(s.h_final.clone())
+        assert int(core.ctx[0]) == 5 * m
+        outs.append(torch.cat(got))
+        s.release()
+    assert torch.equal(outs[0], outs[1])
