@@ -176,7 +176,7 @@ class Rope:
 def rope(table: Rope, xs: list[torch.Tensor], pos: torch.Tensor, outs: list[torch.Tensor] | None = None,
          stream=None) -> list[torch.Tensor]:
     """xs (q and k, up to 4 tensors [T, heads, D] of one type) rotated to pos [T] (int32).
-    outs may be xs itself: rotated in place."""
+    outs may be xs itself: rotated in place. No tensor may be given twice."""
     n = len(xs)
     if not 1 <= n <= 4:
         raise ValueError(f"{n} tensors (1 to 4)")

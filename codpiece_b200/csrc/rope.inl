@@ -125,6 +125,10 @@ extern "C" cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *con
     if (rope->n_dims > d) return fail(CPQ_ERR_INVALID_ARG, "rope: n_dims=%d > head size %lld", rope->n_dims, (long long)d);
     if (d > 4096) return fail(CPQ_ERR_UNSUPPORTED, "rope: head size %lld > 4096", (long long)d);
     if (t == 0) return CPQ_SUCCESS;
+    for (int i = 0; i < n; i++)  // the tensors are rotated at once, by CTAs that do not wait for one another
+        for (int j = 0; j < n; j++)
+            if (i != j && (y[i]->data == y[j]->data || y[i]->data == x[j]->data))
+                return fail(CPQ_ERR_INVALID_ARG, "rope: output %d is also tensor %d", i, j);
     if (!pos) return fail(CPQ_ERR_INVALID_ARG, "rope: null positions");
     const bool half = rope->mode == CPQ_ROPE_HALF;
     // 16-byte items want whole vectors: of each half and of the tail, or of the head

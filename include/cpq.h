@@ -436,7 +436,8 @@ cpq_status cpq_rope_create(const cpq_rope_params *params, cpq_rope **rope);
 void cpq_rope_destroy(cpq_rope *rope);
 /* y[i] = x[i] rotated to positions pos[token] (any int32), for n <= 4 tensors
  * of one type, head size and token count (q and k together). y[i] may be x[i]
- * itself (same data and strides); otherwise the two must not overlap. */
+ * itself (same data and strides); otherwise no output may overlap another
+ * tensor of the call. */
 cpq_status cpq_rope_apply(const cpq_rope *rope, const cpq_tensor *const *x, cpq_tensor *const *y, int n,
                           const int32_t *pos, void *stream);
 

@@ -244,3 +244,18 @@ def test_paged_attn_refuses_out_in_place_of_q(L):
     for name, v in dict(seq_start=0x10, kv_len=0x20, table=0x30, table_stride=8, n_seqs=2, max_blocks=8).items():
         setattr(s, name, v)
     assert L.cpq_paged_attn(C.byref(q), C.byref(c), C.byref(s), 0.1, 1, C.byref(out), None, 0x80000, 1 << 30, None) == INVALID
+
+
+def test_rope_refuses_the_same_output_twice(L):
+    h = C.c_void_p()
+    assert L.cpq_rope_create(C.byref(rope_params(n_dims=64)), C.byref(h)) == OK
+    call = lambda x, y: L.cpq_rope_apply(h, arr(*x), arr(*y), len(x), C.c_void_p(0x9000), None)  # noqa: E731
+    a, b, c = tensor(128, 4, 3), tensor(128, 2, 3, data=0x20000), tensor(128, 4, 3, data=0x30000)
+    assert call([a, a], [a, a]) == INVALID                 # in place, twice
+    assert call([a, a], [c, c]) == INVALID
+    assert call([a, b], [c, tensor(128, 2, 3, data=0x30000)]) == INVALID
+    d = tensor(128, 4, 3, data=0x40000)
+    assert call([a, c], [c, d]) == INVALID                 # one tensor's output is the other's input
+    none = [tensor(128, 4, 0), tensor(128, 4, 0)]
+    assert call(none, none) == OK                          # no tokens: nothing overlaps
+    L.cpq_rope_destroy(h)
