@@ -96,6 +96,16 @@ extern "C" cpq_status cpq_kv_slots(const cpq_kv_slot_args *s, void *stream) {
         return fail(CPQ_ERR_INVALID_ARG, "kv_slots: null per-sequence pointer");
     if (s->n_rows > 0 && (!s->pos || !s->slot)) return fail(CPQ_ERR_INVALID_ARG, "kv_slots: null pos or slot");
     if (s->n_free > 0 && !s->free_pages) return fail(CPQ_ERR_INVALID_ARG, "kv_slots: null free_pages");
+    // CTAs read the inputs while others write the outputs
+    const void *const in[4] = {s->ctx_len, s->new_len, s->free_pages, s->taken};
+    const void *const out[6] = {s->table, s->taken_out, s->seq_start, s->kv_len, s->pos, s->slot};
+    for (int i = 0; i < 6; i++) {
+        for (int j = 0; j < 4; j++)
+            if (out[i] && out[i] == in[j] && !(i == 1 && j == 3))
+                return fail(CPQ_ERR_INVALID_ARG, "kv_slots: an output is also an input (only taken_out may be taken)");
+        for (int j = 0; j < i; j++)
+            if (out[i] && out[i] == out[j]) return fail(CPQ_ERR_INVALID_ARG, "kv_slots: two outputs at one address");
+    }
     SlotArgs a{s->ctx_len, s->new_len, s->n_seqs, s->table, s->table_stride, s->max_blocks, s->block,
                s->free_pages, s->n_free, s->taken, s->taken_out, s->seq_start, s->kv_len, s->pos, s->slot, s->n_rows};
     // a row per thread; the scan, which every CTA repeats, takes longer than that (300 requests, 60000 rows: 6.4 us,

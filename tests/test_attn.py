@@ -259,3 +259,21 @@ def test_rope_refuses_the_same_output_twice(L):
     none = [tensor(128, 4, 0), tensor(128, 4, 0)]
     assert call(none, none) == OK                          # no tokens: nothing overlaps
     L.cpq_rope_destroy(h)
+
+
+def test_kv_slots_refuses_outputs_over_inputs(L):
+    from codpiece_b200._lib import CpqKvSlotArgs
+    base = dict(ctx_len=0x10, new_len=0x20, n_seqs=2, table=0x30, table_stride=4, max_blocks=4, block=16, free_pages=0x40,
+                n_free=3, taken=0x50, taken_out=0x60, seq_start=0x70, kv_len=0x80, pos=0x90, slot=0xa0, n_rows=5)
+
+    def args(**k):
+        a = CpqKvSlotArgs()
+        for name, v in {**base, **k}.items():
+            setattr(a, name, v)
+        return L.cpq_kv_slots(C.byref(a), None)
+
+    outs = ("table", "taken_out", "seq_start", "kv_len", "pos", "slot")
+    for out in outs:
+        for other in ("ctx_len", "new_len", "free_pages", "taken", *outs):
+            if other != out and (out, other) not in (("taken_out", "taken"), ("taken", "taken_out")):
+                assert args(**{out: base[other]}) == INVALID, (out, other)  # lengths advanced in place, for one
