@@ -167,6 +167,7 @@ extern "C" cpq_status cpq_kv_gather(const cpq_kv_cache *c, const int64_t *slot, 
     const int64_t t = k->ne[2];
     if (t == 0) return CPQ_SUCCESS;
     if (!slot) return fail(CPQ_ERR_INVALID_ARG, "kv_gather: null slots");
+    if (k->data == v->data) return fail(CPQ_ERR_INVALID_ARG, "kv_gather: k and v are one tensor");
     const size_t b = size_t(act_bytes(k->type));
     GatherArgs a{};
     cpq_tensor *const y[2] = {k, v};

@@ -277,3 +277,11 @@ def test_kv_slots_refuses_outputs_over_inputs(L):
         for other in ("ctx_len", "new_len", "free_pages", "taken", *outs):
             if other != out and (out, other) not in (("taken_out", "taken"), ("taken", "taken_out")):
                 assert args(**{out: base[other]}) == INVALID, (out, other)  # lengths advanced in place, for one
+
+
+def test_gather_refuses_one_tensor_for_keys_and_values(L):
+    slot, c = C.c_void_p(0x5000), cache()
+    k, v = tensor(256, 4, 3), tensor(256, 4, 3)
+    assert L.cpq_kv_gather(C.byref(c), slot, C.byref(k), C.byref(v), None) == INVALID
+    none = tensor(256, 4, 0)
+    assert L.cpq_kv_gather(C.byref(c), slot, C.byref(none), C.byref(none), None) == OK
