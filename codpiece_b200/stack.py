@@ -83,13 +83,16 @@ class Comm:
 
 
 class AttnCore:
-    """The attention core of a one-GPU stack's layers for one sequence: rotary frequencies, one paged
+    """The attention core of a one-GPU stack's layers for one sequence (attn_q without the gate that
+    q_has_gate stands for, which has no operator here): rotary frequencies, one paged
     8-bit cache per layer, and the block table, page list and length they share (all on the device, so
     a step can be captured and replayed; the length advances by the stack's M tokens per step). A step that
     would pass max_ctx (rounded up to whole blocks) caches nothing, its attention gives zeros, the length stays."""
 
     def __init__(self, hp: tp.Hparams, n_layer: int, max_ctx: int, block: int = 64, fmt: int = attn.KV_INT8,
                  rope: attn.Rope | None = None, device="cuda"):
+        if hp.q_has_gate or hp.head_v != hp.head_k:
+            raise ValueError("the attention core takes q without a gate beside it, and keys and values of one head size")
         dev = torch.device(device)
         pages = -(-max_ctx // block)
         self.block = block
@@ -163,6 +166,12 @@ class Stack:
                 raise ValueError("the attention core runs on one GPU, with per-call layers")
             if len(attn_core.caches) != n_layer:
                 raise ValueError(f"{len(attn_core.caches)} caches for {n_layer} layers")
+            if hp.q_has_gate or hp.head_v != hp.head_k:
+                raise ValueError("the attention core takes q without a gate beside it, and keys and values of one head size")
+            for c in attn_core.caches:
+                if (c.n_head_kv, c.head_dim, c.device) != (hp.n_head_kv, hp.head_k, self.dev):
+                    raise ValueError(f"a cache of {c.n_head_kv} heads of {c.head_dim} on {c.device} for a stack of "
+                                     f"{hp.n_head_kv} of {hp.head_k} on {self.dev}")
             self.ab = f(qmax)
             ints = lambda n, dt=torch.int32: torch.zeros(n, dtype=dt, device=self.dev)  # noqa: E731
             self.new_len = torch.full((1,), m, dtype=torch.int32, device=self.dev)

@@ -285,3 +285,14 @@ def test_gather_refuses_one_tensor_for_keys_and_values(L):
     assert L.cpq_kv_gather(C.byref(c), slot, C.byref(k), C.byref(v), None) == INVALID
     none = tensor(256, 4, 0)
     assert L.cpq_kv_gather(C.byref(c), slot, C.byref(none), C.byref(none), None) == OK
+
+
+def test_attn_core_refuses_gated_queries():
+    """With q_has_gate attn_q gives 2 x 256 rows a head; read as heads of 256 they would be other heads' and gates."""
+    import dataclasses
+
+    from codpiece_b200 import stack, tp
+    with pytest.raises(ValueError, match="gate"):
+        stack.AttnCore(tp.HP_QWEN35_27B, 1, max_ctx=64)
+    with pytest.raises(ValueError, match="head size"):
+        stack.AttnCore(dataclasses.replace(tp.HP_BENCH_27B, head_v=128), 1, max_ctx=64)

@@ -160,3 +160,20 @@ def test_capture_in_mid_sequence_caches_nothing(cuda, m):
         outs.append(torch.cat(got))
         s.release()
     assert torch.equal(outs[0], outs[1])
+
+
+def test_stack_refuses_a_core_of_other_shapes(cuda):
+    import dataclasses
+
+    from codpiece_b200 import attn, stack, tp
+
+    hp = tp.HP_BENCH_27B
+    for other in (dataclasses.replace(hp, n_head_kv=2), dataclasses.replace(hp, head_k=128, head_v=128)):
+        core = stack.AttnCore(other, 1, max_ctx=64, rope=attn.Rope(64))
+        with pytest.raises(ValueError):
+            stack.Stack(hp, n_layer=1, m=1, head=False, attn_core=core)
+    core = _core(stack, tp, attn, 1, max_ctx=64)
+    with pytest.raises(ValueError, match="gate"):
+        stack.Stack(dataclasses.replace(hp, q_has_gate=True), n_layer=1, m=1, head=False, attn_core=core)
+    with pytest.raises(ValueError):
+        stack.AttnCore(dataclasses.replace(hp, q_has_gate=True), 1, max_ctx=64)
