@@ -220,14 +220,16 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
 }
 
 // 16 bytes of codes, or zeros; the load stays in flight (selecting its result
-// afterwards would wait for it).
+// afterwards would wait for it). Not a non-coherent load: the append before may
+// still be writing when this kernel begins.
 __device__ __forceinline__ uint4 ldg_codes(const uint8_t *p, bool there) {
     uint4 r = make_uint4(0, 0, 0, 0);
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
-        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        "@p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
         : "+r"(r.x), "+r"(r.y), "+r"(r.z), "+r"(r.w)
-        : "l"(p), "r"(there ? 1u : 0u));
+        : "l"(p), "r"(there ? 1u : 0u)
+        : "memory");
     return r;
 }
 

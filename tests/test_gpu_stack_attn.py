@@ -177,3 +177,45 @@ def test_stack_refuses_a_core_of_other_shapes(cuda):
         stack.Stack(dataclasses.replace(hp, q_has_gate=True), n_layer=1, m=1, head=False, attn_core=core)
     with pytest.raises(ValueError):
         stack.AttnCore(dataclasses.replace(hp, q_has_gate=True), 1, max_ctx=64)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_after_a_rollback_attention_is_that_of_what_the_cache_holds(cuda, fmt):
+    """Rejected tokens are forgotten: each step after a rollback equals 64-bit attention over the cache's values, and what
+    the rejected tokens leave behind is at most a coarser scale in the last page kept. Its codes are made again once for
+    each rejected token that raises the scale, off by half a step of the new scale each time (int8: the scale; e4m3: at
+    most 2^-4 of the value, or 2^-10 scales for the subnormal codes)."""
+    torch = cuda
+    from codpiece_b200 import attn, stack, tp
+
+    core = _core(stack, tp, attn, 1, max_ctx=128, block=32, fmt=fmt)
+    s = stack.Stack(tp.HP_BENCH_27B, n_layer=1, m=1, seed=5, head=False, attn_core=core)
+    cache = core.caches[0]
+    xs = torch.randn(60, 1, 5120, device="cuda", generator=torch.Generator("cuda").manual_seed(7))
+
+    def step(x):
+        s.h.copy_(x)
+        s.step_body()
+        kv = int(core.ctx[0])
+        ref = _dense(torch, attn, s.qb.view(1, 24, 256), cache, core, kv)
+        assert float((s.ab.view(1, 24, 256).double() - ref).norm() / ref.norm()) <= 1e-5
+
+    def held():
+        slots = torch.tensor([int(core.table[0, p // 32]) * 32 + p % 32 for p in range(45)], device="cuda")
+        return attn.kv_gather(cache, slots)
+
+    for x in xs[:45]:
+        step(x)
+    before, rejected = held(), 8
+    for x in xs[45:45 + rejected]:
+        step(x)
+    core.rollback(rejected)
+    assert int(core.ctx[0]) == 45 and int(core.taken[0]) == 2
+    last = int(core.table[0, 1])
+    for now, was, scale in zip(held(), before, (cache.k_scale[last], cache.v_scale[last])):
+        assert torch.equal(now[:32], was[:32])                     # full pages are not touched
+        half = scale[None, :, None] / 2 if fmt == 0 else torch.maximum(was[32:].abs() / 16, scale[None, :, None] * 2.0 ** -10)
+        assert ((now[32:] - was[32:]).abs() <= 1.1 * rejected * half).all()  # (1.1: e4m3's values drift between codings)
+    for x in xs[45 + rejected:]:
+        step(x)
+    s.release()
