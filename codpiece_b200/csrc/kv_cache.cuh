@@ -63,7 +63,7 @@ __device__ __forceinline__ void slot_scan(int64_t &a, int64_t &b, int64_t (*part
 // the table where the request held that block before, from the free list
 // otherwise, so no CTA reads what another writes. `taken` is read by every CTA
 // and written by CTA 0, hence one CTA when taken_out is taken (the host's
-// choice). Latency: 16 decode requests 5.2 us, 300 requests with 60000 rows 6.4.
+// choice). Latency: 16 decode requests 5.2 us, 300 requests with 60000 rows 6.4 (72 with one CTA).
 __global__ void __launch_bounds__(kSlotThreads) kv_slots_kernel(const SlotArgs a) {
     __shared__ int64_t part[32][2];
     __shared__ int s_start[kSlotThreads + 1];  // the chunk's first rows (clipped to n_rows)
@@ -346,6 +346,9 @@ struct AppendArgs {
 // two passes over a run in shared memory bound it (68 % of issue slots), not its
 // bytes. 64 threads per 8 KB: with twice as many 39 us, with half 36 (fp32 57, 34).
 // 40 registers instead of 48 (a few spilled outside the loops): 3 to 9 % less.
+// These are calls in which no scale grows; where one does, the page's rows are
+// coded again, a 64-bit division per code (24 rows, fp32 to int8, pages of 64: 3.1
+// us, 24 with an eighth of the pages growing, 31 with all of them).
 constexpr int kAppendMaxGroup = 32;
 
 template <typename T, bool WIDE, int FMT>

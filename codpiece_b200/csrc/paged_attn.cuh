@@ -336,12 +336,12 @@ __device__ __forceinline__ float attn_lse(float ref, float sum) {
 // the others a quarter of their registers (warps are allotted in fours): with
 // one, the accumulators of D = 256 spilled.
 //
-// Measured (24 heads over 4 of 256): 1 request over 100003 keys, fp32, 53.5 us
-// (3.8 TB/s of codes, 0.59 of a measured copy; 38 % of issue slots, 26 % of the
+// Measured (24 heads over 4 of 256): 1 request over 100003 keys, fp32, 54.1 us
+// (3.8 TB/s of codes, 0.58 of a measured copy; 37 % of issue slots, 25 % of the
 // tensor pipe: a warp's tile is a chain of loads, conversions and MMAs, two warps a
 // scheduler cannot hide all of it, and registers allow no third); 32
 // ragged bf16 requests of up to 16000 keys 133 us (4.35 TB/s, 0.67); 1 request over
-// 1000 keys 13.6, most of it beginning and joining.
+// 1000 keys 13.9, most of it beginning and joining.
 //
 // Operand order. A key tile's codes go from shared memory to the MMA's B
 // registers without a transpose:

@@ -46,10 +46,12 @@
 // for anything else (6 of 15 cycles per instruction; 8000 cycles per key tile).
 // Masked tiles therefore get their -inf written into S beforehand.
 //
-// Measured (24 heads over 4 of 256): 1024 bf16 tokens behind 16384 keys 510 us
-// (783 TFLOP/s, 0.48 of a measured GEMM; 478 us at a cool clock: 69 % of issue
-// slots, 43 % of the tensor pipe), three fp32 chunks of up to 700 over up to 9000
-// keys, twice the products, 615 us (943 TFLOP/s of fp16 products, 0.57). Issue slots
+// Measured (24 heads over 4 of 256): 1024 bf16 tokens behind 16384 keys 522 us
+// (765 TFLOP/s, 0.47 of a measured GEMM; 491 us at a cool clock: 69 % of issue
+// slots, 43 % of the tensor pipe; 547 in a long loop, at the power cap), three fp32
+// chunks of up to 700 over up to 9000 keys, twice the products, 618 us (940 TFLOP/s
+// of fp16 products, 0.57).
+// Following each row's contributions instead of its scores cost 2 % of the first. Issue slots
 // bound it, conversion and softmax together; S and P V as pairs of SMs would halve
 // the conversions, which all CTAs of a head's row tiles repeat.
 //

@@ -104,7 +104,9 @@ class AttnCore:
         self.taken, self.ctx = i32(0), i32(0)
 
     def rollback(self, n: int | torch.Tensor) -> None:
-        """Forgets the last n tokens (rejected by a verify step): their pages go back to the list."""
+        """Forgets the last n tokens (rejected by a verify step): their pages go back to the list. A page
+        scale that they raised stays raised, and the codes of the tokens kept in that page stay as they
+        were made again for it: these may be off by half a step of the raised scale for each time it rose."""
         self.ctx.sub_(n).clamp_(min=0)
         self.taken.copy_((self.ctx + (self.block - 1)) // self.block)
 

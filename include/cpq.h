@@ -403,7 +403,7 @@ cpq_status cpq_gated_delta_net(const cpq_tensor *q, const cpq_tensor *k, const c
  *
  * What stands between the q/k/v projections and attn_output in an attention
  * layer (qwen35.rs:3000-3197: ggml_rope_multi, the cache writes,
- * ggml_flash_attn_ext), for many requests of different lengths whose keys and
+ * ggml_flash_attn_ext; not the norms of q and k, nor the gate beside q), for many requests of different lengths whose keys and
  * values live in pages of one pool. A step is cpq_kv_slots once, then per
  * layer cpq_rope_apply on q and k, cpq_kv_append, cpq_paged_attn. Lengths,
  * tables and slots stay on the device, so a step can be captured in a CUDA
@@ -471,8 +471,8 @@ typedef struct cpq_kv_cache {
  * served (too few free pages left, more than max_blocks blocks, rows past
  * n_rows, a negative length) keeps its rows' place but gets kv_len 0, slots -1
  * and no page; requests that need no page are served even then. Outputs must
- * not overlap inputs, except table (in and out) and taken_out, which may be
- * taken itself. */
+ * not overlap inputs or one another, except table (in and out) and taken_out,
+ * which may be taken itself (one CTA then places all rows). */
 typedef struct cpq_kv_slot_args {
     const int32_t *ctx_len, *new_len; /* [n_seqs] */
     int64_t n_seqs;
@@ -497,7 +497,10 @@ cpq_status cpq_kv_slots(const cpq_kv_slot_args *args, void *stream);
  * to fp32, or the old scale if that is larger and the run does not begin at
  * the page's first place; codes are x / s rounded to nearest, ties to even.
  * When s grows, the places before the run are coded again (c * s_old / s to
- * nearest); the places after it are left as they are. NaN is stored as 0,
+ * nearest); the codes after it are left as they are, for places that will be
+ * written again. A scale does not shrink before its page is begun anew, so
+ * tokens taken back leave a scale that they raised. A page is begun at its
+ * first place: until then its scale is whatever the memory holds. NaN is stored as 0,
  * infinities as the largest code, and neither counts for the scale; a scale
  * under 2^-100 becomes 0. All rows of a call that go to one page must form one
  * run: two runs in a page in one call leave it undefined. */
