@@ -398,14 +398,16 @@ class Stack:
         attention core a step of no tokens, which leaves its cache and length as they are)."""
         if self.attn is not None:
             self.new_len.zero_()
-        s = torch.cuda.Stream(device=self.dev)
-        s.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(s):
-            self.step_body()
-        torch.cuda.current_stream().wait_stream(s)
-        torch.cuda.synchronize(self.dev)
-        if self.attn is not None:
-            self.new_len.fill_(self.m)
+        try:
+            s = torch.cuda.Stream(device=self.dev)
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                self.step_body()
+            torch.cuda.current_stream().wait_stream(s)
+            torch.cuda.synchronize(self.dev)
+        finally:
+            if self.attn is not None:
+                self.new_len.fill_(self.m)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             self.step_body()

@@ -219,3 +219,18 @@ def test_after_a_rollback_attention_is_that_of_what_the_cache_holds(cuda, fmt):
     for x in xs[45 + rejected:]:
         step(x)
     s.release()
+
+
+def test_a_capture_that_fails_leaves_the_steps_their_tokens(cuda, monkeypatch):
+    from codpiece_b200 import attn, stack, tp
+
+    core = _core(stack, tp, attn, 1, max_ctx=64)
+    s = stack.Stack(tp.HP_BENCH_27B, n_layer=1, m=2, head=False, attn_core=core)
+    with monkeypatch.context() as mp:
+        mp.setattr(attn, "rope", lambda *a, **k: (_ for _ in ()).throw(RuntimeError("on the host")))
+        with pytest.raises(RuntimeError, match="on the host"):
+            s.capture()
+    assert int(core.ctx[0]) == 0
+    s.step_body()
+    assert int(core.ctx[0]) == 2
+    s.release()
